@@ -153,6 +153,25 @@ typedef struct {
  * pool's split-K scratch). */
 VW_API int32_t vw_paged_decode(vw_pool* pool, const vw_decode_args* args, void* stream);
 
+/* Sliding-window attention with sinks (no reference kernel).  A query at
+ * position p sees the keys j <= p with p - j < window or j < sinks: the last
+ * `window` tokens, itself among them, and the first `sinks` tokens.  window
+ * must be > 0; a window of the sequence's length or more sees everything.
+ * Pages without a visible key are neither resolved nor read, so their
+ * block-table entries may hold anything (e.g. ids of blocks given back).
+ * Every row sees its own token, so no row is empty. */
+typedef struct {
+    uint32_t window;
+    uint32_t sinks;
+} vw_window;
+
+/* vw_paged_decode under such a window: same arguments, flags (all but
+ * VW_DECODE_PLANNED), fused append and results otherwise, over every pool kind.
+ * A hidden token's V row may hold anything, Inf and NaN included.  The split
+ * over the GPU is over the visible pages alone. */
+VW_API int32_t vw_paged_decode_window(vw_pool* pool, const vw_decode_args* args, const vw_window* window,
+                                      void* stream);
+
 /* Page assignment of a decode batch, computed once and reused by every layer's
  * vw_paged_decode with VW_DECODE_PLANNED (no counterpart in the reference,
  * whose decode has one CTA per sequence): each decode CTA's range of pages, its
@@ -226,6 +245,9 @@ typedef struct {
     float rope_theta;              /* > 0: fused RoPE on q and the new K rows (VW_DECODE_ROPE) */
 } vw_step_host_args;
 VW_API int32_t vw_decode_step_host(vw_pool* pool, const vw_step_host_args* args, void* stream);
+/* The same step with every layer's decode under one window. */
+VW_API int32_t vw_decode_step_host_window(vw_pool* pool, const vw_step_host_args* args,
+                                          const vw_window* window, void* stream);
 
 /* ---- Chunked prefill over the pool ------------------------------------------
  * Replaces: launch_flash_attn_prefill (kernels/attention/flash_attention.bm:167-177,
@@ -264,6 +286,13 @@ typedef struct {
 #define VW_PREFILL_PDL 0x4u        /* launch as a programmatic dependent of the previous kernel */
 
 VW_API int32_t vw_paged_prefill(vw_pool* pool, const vw_prefill_args* args, void* stream);
+/* vw_paged_prefill under a sliding window with sinks (vw_window), which needs
+ * VW_PREFILL_CAUSAL.  The chunk's append writes every row as before.  Pages
+ * that no query of a 128-token tile sees are not read.  V rows that no query of
+ * a tile sees may hold anything; one that another query of its tile sees must
+ * be finite, as in vw_paged_prefill. */
+VW_API int32_t vw_paged_prefill_window(vw_pool* pool, const vw_prefill_args* args, const vw_window* window,
+                                       void* stream);
 
 /* ---- FP8 weight path sharing the KV codec ---------------------------------------
  * rms_norm_fp8_out (kernels/norm/rms_norm.bm:62-94): x, weight f16
@@ -414,13 +443,14 @@ VW_API const char* vw_last_error(void);
  * one kind (count 0 disarms); each later call of an entry point that can fail
  * that way consumes one and returns the status at once, before touching the
  * device or the bookkeeping:
- *   VW_FAULT_OOM         -> VW_ERR_OOM: vw_pool_create, vw_decode_step_host,
+ *   VW_FAULT_OOM         -> VW_ERR_OOM: vw_pool_create, vw_decode_step_host(_window),
  *                           voidweb_forward_pass, vw_bm_alloc, vw_bm_alloc_seq, vw_bm_cow
  *   VW_FAULT_INVALID_ARG -> VW_ERR_INVALID_ARG and
  *   VW_FAULT_CUDA        -> VW_ERR_CUDA: vw_pool_create, vw_kv_append,
- *                           vw_paged_decode, vw_paged_decode_static, vw_decode_plan,
- *                           vw_block_copy, vw_kv_gather, vw_paged_prefill,
- *                           vw_decode_step_host, voidweb_forward_pass,
+ *                           vw_paged_decode(_window), vw_paged_decode_static,
+ *                           vw_decode_plan, vw_block_copy, vw_kv_gather,
+ *                           vw_paged_prefill(_window),
+ *                           vw_decode_step_host(_window), voidweb_forward_pass,
  *                           vw_rms_norm_fp8_out, vw_gemm_fp8
  * The environment variable VOIDWEB_KV_FAULT ("oom:N,invalid:N,cuda:N") arms
  * the same counts when the library is loaded.  No counterpart in the reference. */

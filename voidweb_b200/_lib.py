@@ -67,6 +67,10 @@ class PrefillArgs(ctypes.Structure):
                 ("out", vp), ("scale", f32), ("rope_theta", f32)]
 
 
+class Window(ctypes.Structure):
+    _fields_ = [("window", u32), ("sinks", u32)]
+
+
 class SchedConfig(ctypes.Structure):
     _fields_ = [("max_batch_tokens", u32), ("max_running_seqs", u32), ("max_chunk", u32),
                 ("max_seq_len", u32), ("prefix_cache", u32), ("reserved", u32)]
@@ -113,7 +117,9 @@ SIGNATURES = {
     "vw_pool_check": (i32, [vp, ctypes.POINTER(u32)]),
     "vw_kv_append": (i32, [vp, u32, vp, vp, vp, u32, vp]),
     "vw_paged_decode": (i32, [vp, ctypes.POINTER(DecodeArgs), vp]),
+    "vw_paged_decode_window": (i32, [vp, ctypes.POINTER(DecodeArgs), ctypes.POINTER(Window), vp]),
     "vw_paged_prefill": (i32, [vp, ctypes.POINTER(PrefillArgs), vp]),
+    "vw_paged_prefill_window": (i32, [vp, ctypes.POINTER(PrefillArgs), ctypes.POINTER(Window), vp]),
     "vw_rms_norm_fp8_out": (i32, [vp, vp, vp, u32, u32, f32, f32, vp]),
     "vw_gemm_fp8": (i32, [vp, vp, vp, vp, u32, u32, u32, f32, f32, vp]),
     "vw_fp8_weight_check": (i32, [ctypes.POINTER(u32)]),
@@ -129,6 +135,7 @@ SIGNATURES = {
     "vw_block_copy": (i32, [vp, vp, u32, vp]),
     "vw_kv_gather": (i32, [vp, u32, vp, u32, vp, vp, vp, vp, vp]),
     "vw_decode_step_host": (i32, [vp, ctypes.POINTER(StepHostArgs), vp]),
+    "vw_decode_step_host_window": (i32, [vp, ctypes.POINTER(StepHostArgs), ctypes.POINTER(Window), vp]),
     "vw_bm_create": (i32, [u32, u32, ctypes.POINTER(vp)]),
     "vw_bm_destroy": (i32, [vp]),
     "vw_bm_capacity": (u32, [vp]),

@@ -109,12 +109,12 @@ EncodeTiledFn encode_fn() {
 
 // Everything a recorded host-buffer step depends on.
 struct StepKey {
-    uint32_t B, Hq, stride, scale_bits, theta_bits;
+    uint32_t B, Hq, stride, scale_bits, theta_bits, window, sinks;
     const void *q, *k, *v, *bt, *sl, *out;
     const uint8_t* stage;
     bool operator==(const StepKey& o) const {
         return B == o.B && Hq == o.Hq && stride == o.stride && scale_bits == o.scale_bits &&
-               theta_bits == o.theta_bits && q == o.q && k == o.k && v == o.v && bt == o.bt &&
+               theta_bits == o.theta_bits && window == o.window && sinks == o.sinks && q == o.q && k == o.k && v == o.v && bt == o.bt &&
                sl == o.sl && out == o.out && stage == o.stage;
     }
 };
@@ -404,7 +404,7 @@ static int32_t decode_validate(const vw_pool* pool, const vw_decode_args* a) {
                     a->num_q_heads / g.num_kv_heads);
     if (a->block_table_stride == 0)
         return fail(VW_ERR_INVALID_ARG, "vw_paged_decode: block_table_stride must be > 0");
-    if (!a->q || !a->block_tables || !a->seq_lens || !a->out)
+    if (a->num_seqs && (!a->q || !a->block_tables || !a->seq_lens || !a->out))
         return fail(VW_ERR_INVALID_ARG, "vw_paged_decode: null device pointer");
     if ((a->k_new == nullptr) != (a->v_new == nullptr))
         return fail(VW_ERR_INVALID_ARG, "vw_paged_decode: k_new and v_new go together");
@@ -413,6 +413,18 @@ static int32_t decode_validate(const vw_pool* pool, const vw_decode_args* a) {
         return fail(VW_ERR_INVALID_ARG, "vw_paged_decode: misaligned pointer");
     if (!(a->scale >= 0.0f) || std::isinf(a->scale))
         return fail(VW_ERR_INVALID_ARG, "vw_paged_decode: bad scale");
+    return VW_OK;
+}
+
+// A window as a launch takes it: positions stay below kMaxWindow, so a larger
+// window or sink count means the same as kMaxWindow.  Null: no window.
+static vw_window clamp_window(const vw_window* w) {
+    return w ? vw_window{std::min(w->window, kMaxWindow), std::min(w->sinks, kMaxWindow)} : vw_window{0, 0};
+}
+
+static int32_t window_validate(const vw_window* w, const char* what) {
+    if (!w) return fail(VW_ERR_INVALID_ARG, "%s: null window", what);
+    if (w->window == 0) return fail(VW_ERR_INVALID_ARG, "%s: window must be > 0", what);
     return VW_OK;
 }
 
@@ -453,7 +465,7 @@ uint32_t segment_cost(const PoolGeom& g) {
 }
 
 static int32_t decode_launch(vw_pool* pool, const vw_decode_args* a, cudaStream_t s,
-                             const DecodeScratch* fixed = nullptr) {
+                             const DecodeScratch* fixed = nullptr, const vw_window* window = nullptr) {
     const PoolGeom& g = pool->geom;
     DecodeLaunch L{};
     DecodeParams& p = L.p;
@@ -489,6 +501,9 @@ static int32_t decode_launch(vw_pool* pool, const vw_decode_args* a, cudaStream_
     const float scale = a->scale > 0.0f ? a->scale : 1.0f / std::sqrt((float)g.head_dim);
     p.scale_log2 = scale * 1.4426950408889634f;
     p.rope_theta = (a->flags & VW_DECODE_ROPE) ? a->rope_theta : 0.0f;
+    const vw_window win = clamp_window(window);
+    p.window = win.window;
+    p.sinks = win.sinks;
     p.wait_cycles = pool->wait_cycles;
     if (pool->wait_cycles) {
         // the bounded-wait test hook: the query tiles are withheld (and read only
@@ -512,6 +527,20 @@ int32_t vw_paged_decode(vw_pool* pool, const vw_decode_args* args, void* stream)
     if (args->num_seqs == 0) return VW_OK;
     DeviceScope ds(pool->cfg.device);
     return decode_launch(pool, args, static_cast<cudaStream_t>(stream));
+}
+
+int32_t vw_paged_decode_window(vw_pool* pool, const vw_decode_args* args, const vw_window* window,
+                               void* stream) {
+    VW_FAULT_POINT(kFaultLaunch, "vw_paged_decode_window");
+    int32_t rc = decode_validate(pool, args);
+    if (rc == VW_OK) rc = window_validate(window, "vw_paged_decode_window");
+    if (rc != VW_OK) return rc;
+    // a plan assigns every page of the batch, a windowed launch the visible ones
+    if (args->flags & VW_DECODE_PLANNED)
+        return fail(VW_ERR_INVALID_ARG, "vw_paged_decode_window: VW_DECODE_PLANNED does not go with a window");
+    if (args->num_seqs == 0) return VW_OK;
+    DeviceScope ds(pool->cfg.device);
+    return decode_launch(pool, args, static_cast<cudaStream_t>(stream), nullptr, window);
 }
 
 // ---------------------------------------------------------------------------
@@ -538,7 +567,7 @@ static int32_t prefill_validate(const vw_pool* pool, const vw_prefill_args* a) {
         return fail(VW_ERR_INVALID_ARG, "vw_paged_prefill: block_table_stride must be > 0");
     if (a->num_tokens > (1u << 24) || (uint64_t)a->num_tokens * g.num_kv_heads >= (1ull << 31))
         return fail(VW_ERR_INVALID_ARG, "vw_paged_prefill: num_tokens %u too large", a->num_tokens);
-    if (!a->q || !a->cu_seqlens || !a->ctx_start || !a->block_tables || !a->out)
+    if (a->num_seqs && a->num_tokens && (!a->q || !a->cu_seqlens || !a->ctx_start || !a->block_tables || !a->out))
         return fail(VW_ERR_INVALID_ARG, "vw_paged_prefill: null device pointer");
     if ((a->k_new == nullptr) != (a->v_new == nullptr))
         return fail(VW_ERR_INVALID_ARG, "vw_paged_prefill: k_new and v_new go together");
@@ -551,10 +580,7 @@ static int32_t prefill_validate(const vw_pool* pool, const vw_prefill_args* a) {
     return VW_OK;
 }
 
-int32_t vw_paged_prefill(vw_pool* pool, const vw_prefill_args* a, void* stream) {
-    VW_FAULT_POINT(kFaultLaunch, "vw_paged_prefill");
-    int32_t rc = prefill_validate(pool, a);
-    if (rc != VW_OK) return rc;
+static int32_t prefill_launch(vw_pool* pool, const vw_prefill_args* a, void* stream, const vw_window* window) {
     if (a->num_seqs == 0 || a->num_tokens == 0) return VW_OK;
     DeviceScope ds(pool->cfg.device);
     const PoolGeom& g = pool->geom;
@@ -592,6 +618,9 @@ int32_t vw_paged_prefill(vw_pool* pool, const vw_prefill_args* a, void* stream) 
     const float scale = a->scale > 0.0f ? a->scale : 1.0f / std::sqrt((float)g.head_dim);
     p.scale_log2 = scale * 1.4426950408889634f;
     p.rope_theta = theta;
+    const vw_window win = clamp_window(window);
+    p.window = win.window;
+    p.sinks = win.sinks;
     p.wait_cycles = pool->wait_cycles;
     L.tmap = &pool->tmap_half;
     L.head_dim = g.head_dim;
@@ -601,6 +630,24 @@ int32_t vw_paged_prefill(vw_pool* pool, const vw_prefill_args* a, void* stream) 
     e = launch_paged_prefill(L);
     if (e != cudaSuccess) return cuda_fail(e, "vw_paged_prefill: launch");
     return VW_OK;
+}
+
+int32_t vw_paged_prefill(vw_pool* pool, const vw_prefill_args* a, void* stream) {
+    VW_FAULT_POINT(kFaultLaunch, "vw_paged_prefill");
+    int32_t rc = prefill_validate(pool, a);
+    return rc != VW_OK ? rc : prefill_launch(pool, a, stream, nullptr);
+}
+
+int32_t vw_paged_prefill_window(vw_pool* pool, const vw_prefill_args* a, const vw_window* window,
+                                void* stream) {
+    VW_FAULT_POINT(kFaultLaunch, "vw_paged_prefill_window");
+    int32_t rc = prefill_validate(pool, a);
+    if (rc == VW_OK) rc = window_validate(window, "vw_paged_prefill_window");
+    if (rc != VW_OK) return rc;
+    // the window ends at the query's own position
+    if (!(a->flags & VW_PREFILL_CAUSAL))
+        return fail(VW_ERR_INVALID_ARG, "vw_paged_prefill_window: a window needs VW_PREFILL_CAUSAL");
+    return prefill_launch(pool, a, stream, window);
 }
 
 // ---------------------------------------------------------------------------
@@ -731,7 +778,8 @@ int32_t vw_kv_gather(vw_pool* pool, uint32_t layer, const uint32_t* block_table,
 //    after the kernels); one graph launch replaces the 2 L kernel launches.
 // ---------------------------------------------------------------------------
 
-static int32_t enqueue_step_host(vw_pool* pool, const vw_step_host_args* a, cudaStream_t cs, bool graph) {
+static int32_t enqueue_step_host(vw_pool* pool, const vw_step_host_args* a, const vw_window* window,
+                                 cudaStream_t cs, bool graph) {
     const PoolGeom& g = pool->geom;
     const uint32_t B = a->num_seqs, Hq = a->num_q_heads, L = g.num_layers, D = g.head_dim;
     const size_t qb = (size_t)B * Hq * D * 2, kb = (size_t)B * g.num_kv_heads * D * 2;
@@ -814,7 +862,7 @@ static int32_t enqueue_step_host(vw_pool* pool, const vw_step_host_args* a, cuda
             da.rope_theta = a->rope_theta;
         }
         rc = decode_validate(pool, &da);
-        if (rc == VW_OK) rc = decode_launch(pool, &da, cs);
+        if (rc == VW_OK) rc = decode_launch(pool, &da, cs, nullptr, window);
         if (rc == VW_OK && l + 1 == back[r + 1]) {       // read back a finished group
             const uint32_t l0 = back[r];
             cudaEventRecord(pool->ev_done[r], cs);
@@ -831,8 +879,7 @@ static int32_t enqueue_step_host(vw_pool* pool, const vw_step_host_args* a, cuda
     return rc;
 }
 
-int32_t vw_decode_step_host(vw_pool* pool, const vw_step_host_args* a, void* stream) {
-    VW_FAULT_POINT(kFaultAll, "vw_decode_step_host");
+static int32_t step_host(vw_pool* pool, const vw_step_host_args* a, const vw_window* window, void* stream) {
     if (!pool || !a) return fail(VW_ERR_INVALID_ARG, "vw_decode_step_host: null argument");
     if (a->reserved) return fail(VW_ERR_INVALID_ARG, "vw_decode_step_host: reserved");
     if (a->rope_theta != 0.0f && !(a->rope_theta > 1.0f && std::isfinite(a->rope_theta)))
@@ -868,7 +915,8 @@ int32_t vw_decode_step_host(vw_pool* pool, const vw_step_host_args* a, void* str
     uint32_t sb, tb;
     std::memcpy(&sb, &a->scale, 4);
     std::memcpy(&tb, &a->rope_theta, 4);
-    const StepKey key{B, Hq, a->block_table_stride, sb, tb, a->q, a->k_new, a->v_new,
+    const vw_window win = clamp_window(window);
+    const StepKey key{B, Hq, a->block_table_stride, sb, tb, win.window, win.sinks, a->q, a->k_new, a->v_new,
                       a->block_tables, a->seq_lens, a->out, pool->stage};
     if (!(pool->step_exec && key == pool->step_key) && key == pool->step_seen && !(key == pool->step_bad)) {
         // second call with these arguments: record the step once
@@ -877,7 +925,7 @@ int32_t vw_decode_step_host(vw_pool* pool, const vw_step_host_args* a, void* str
         int32_t rc = VW_ERR_CUDA;
         cudaGraph_t graph = nullptr;
         if (cudaStreamBeginCapture(pool->s_cap, cudaStreamCaptureModeThreadLocal) == cudaSuccess) {
-            rc = enqueue_step_host(pool, a, pool->s_cap, true);
+            rc = enqueue_step_host(pool, a, window, pool->s_cap, true);
             if (cudaStreamEndCapture(pool->s_cap, &graph) != cudaSuccess) rc = VW_ERR_CUDA;
         }
         if (rc == VW_OK && graph &&
@@ -897,12 +945,24 @@ int32_t vw_decode_step_host(vw_pool* pool, const vw_step_host_args* a, void* str
         return VW_OK;
     }
     pool->step_seen = key;
-    int32_t rc = enqueue_step_host(pool, a, cs, false);
+    int32_t rc = enqueue_step_host(pool, a, window, cs, false);
     e = cudaStreamSynchronize(cs);
     if (rc != VW_OK) return rc;
     if (e != cudaSuccess) return cuda_fail(e, "vw_decode_step_host");
     e = cudaGetLastError();
     return e == cudaSuccess ? VW_OK : cuda_fail(e, "vw_decode_step_host");
+}
+
+int32_t vw_decode_step_host(vw_pool* pool, const vw_step_host_args* a, void* stream) {
+    VW_FAULT_POINT(kFaultAll, "vw_decode_step_host");
+    return step_host(pool, a, nullptr, stream);
+}
+
+int32_t vw_decode_step_host_window(vw_pool* pool, const vw_step_host_args* a, const vw_window* window,
+                                   void* stream) {
+    VW_FAULT_POINT(kFaultAll, "vw_decode_step_host_window");
+    const int32_t rc = window_validate(window, "vw_decode_step_host_window");
+    return rc != VW_OK ? rc : step_host(pool, a, window, stream);
 }
 
 // ---------------------------------------------------------------------------

@@ -57,6 +57,7 @@
 #include "vw_internal.h"
 #include "vw_ptx.cuh"
 #include "vw_rope.cuh"
+#include "vw_window.cuh"
 
 #ifndef VW_DECODE_WARPS
 #define VW_DECODE_WARPS 4
@@ -333,10 +334,12 @@ __device__ __forceinline__ void set_err(uint32_t* err, uint32_t bit) { atomicOr(
 // Pages per sequence -> exclusive prefixes of pages (pfx) and of sequences with
 // pages (nzp), by one warp, 32 sequences at a time, keeping each seq_len in
 // slen when given.  A seq_len of 0 gives no pages and one longer than its
-// block-table row is clamped to the row; both are flagged when `report`.
+// block-table row is clamped to the row; both are flagged when `report`.  With
+// WIN only the pages that the window and the sinks leave visible count.
+template <bool WIN>
 __device__ __forceinline__ void warp_prefixes(const uint32_t* seq_lens, int B, int bt_stride,
                                               uint32_t* err, bool report, int* pfx, int* nzp,
-                                              int* slen, int lane) {
+                                              int* slen, int lane, uint32_t window, uint32_t sinks) {
     int run = 0, run_nz = 0;
     if (lane == 0) { pfx[0] = 0; nzp[0] = 0; }
     for (int base_b = 0; base_b < B; base_b += 32) {
@@ -350,6 +353,7 @@ __device__ __forceinline__ void warp_prefixes(const uint32_t* seq_lens, int B, i
                 if (report) set_err(err, kDevErrSeqLen);
                 np = sl <= 0 ? 0 : bt_stride;
             }
+            if (WIN && np > 0) np = decode_span(sl, bt_stride, window, sinks).n;
         }
         int incl = np, incl_nz = np > 0 ? 1 : 0;
 #pragma unroll
@@ -383,6 +387,7 @@ struct Resolved {
 
 // Lane-parallel resolution of CTA-relative page i: its segment, KV head and
 // block id (the block-table load is consumed one batch later).
+template <bool WIN>
 __device__ __forceinline__ Resolved resolve_page(const DecodeParams& p, const Smem& sm, int begin,
                                                  int first_ord, int i, int n) {
     Resolved r{0, -1, -1, -1, 0xFFFFFFFFu, false};
@@ -394,7 +399,8 @@ __device__ __forceinline__ Resolved resolve_page(const DecodeParams& p, const Sm
         const int h = rr / np, pg = rr - h * np;
         r.h = h;
         r.live = true;
-        r.blk = __ldg(p.block_tables + (size_t)b * p.bt_stride + pg);
+        const int lp = WIN ? decode_span(sm.slen[b], (int)p.bt_stride, p.window, p.sinks).page(pg) : pg;
+        r.blk = __ldg(p.block_tables + (size_t)b * p.bt_stride + lp);
         if (i == 0 || pg == 0) {
             r.qseg = sm.nzp[b] * (int)p.Hkv + h - first_ord;
             r.qrow = (int)(b * p.Hq + h * p.group);
@@ -409,7 +415,7 @@ __device__ __forceinline__ Resolved resolve_page(const DecodeParams& p, const Sm
 // record buffer, and its lanes 0 .. IPW-1 issue the pages of issuers
 // lane * PW + pw.  Lane 0 of warp 0 also issues the query tiles, in segment
 // order.
-template <class T>
+template <class T, bool WIN>
 __device__ void producer(const CUtensorMap* tmap, const DecodeParams& p, const Smem& sm,
                          int begin, int n, int first_ord, int pw, uint64_t deadline) {
     const int lane = threadIdx.x & 31;
@@ -475,7 +481,7 @@ __device__ void producer(const CUtensorMap* tmap, const DecodeParams& p, const S
 
     if (lane == 0) VW_TRACE(10, globaltimer());
     if (p.plan == nullptr) {                        // else batch 0 came with the plan
-        Resolved cur = resolve_page(p, sm, begin, first_ord, lane, n);
+        Resolved cur = resolve_page<WIN>(p, sm, begin, first_ord, lane, n);
         publish(cur, 0);
     }
     __syncwarp();
@@ -504,7 +510,7 @@ __device__ void producer(const CUtensorMap* tmap, const DecodeParams& p, const S
     if (p.flags & kDecodePdl) griddep_wait();
     int buf = 0;
     for (int i0 = 0; i0 < n; i0 += 32) {
-        const Resolved nxt = resolve_page(p, sm, begin, first_ord, i0 + 32 + lane, n);
+        const Resolved nxt = resolve_page<WIN>(p, sm, begin, first_ord, i0 + 32 + lane, n);
         const int m = min(32, n - i0);
         if (lane < T::IPW) {
             // the query lane scans every page of the batch for segment starts so
@@ -755,14 +761,14 @@ __device__ __forceinline__ void append_row(const DecodeParams& p, uint8_t* stage
     }
 }
 
-// Zero V rows [valid, 16) of a staged page-head so masked tokens cannot inject
+// Zero V rows [from, to) of a staged page-head so masked tokens cannot inject
 // NaN/Inf through 0 * garbage in the P.V product.
 template <class T>
-__device__ __forceinline__ void zero_tail(uint8_t* stage, int valid, int lane) {
+__device__ __forceinline__ void zero_rows(uint8_t* stage, int from, int to, int lane) {
     const int per_row = T::CHUNKS * 8;                   // 16-B pieces per row
-    const int total = (16 - valid) * per_row;
+    const int total = (to - from) * per_row;
     for (int k = lane; k < total; k += 32) {
-        const int piece = k % per_row, row = 16 + valid + k / per_row;
+        const int piece = k % per_row, row = 16 + from + k / per_row;
         const int c = piece >> 3, ch = piece & 7;
         *reinterpret_cast<uint4*>(stage + c * 4096 + row * 128 + (ch << 4)) = make_uint4(0, 0, 0, 0);
     }
@@ -829,7 +835,7 @@ __device__ __forceinline__ int merge_col(int d) {
     return T::KV == kFP8 ? d ^ ((d >> 4) & 7) : d;
 }
 
-template <class T>
+template <class T, bool WIN>
 __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int end,
                          uint64_t deadline) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -859,6 +865,8 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
         const bool complete = pg0 == 0 && cnt == np;
         const int i_base = x - begin;
         const int seq_len = sm.slen[b];     // read in the prologue: no load after the release
+        PageSpan span{};
+        if constexpr (WIN) span = decode_span(seq_len, (int)p.bt_stride, p.window, p.sinks);
 
         // query tile of this segment (staged by the producer)
         uint32_t qf[T::NT][T::KT][2];
@@ -942,17 +950,24 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
             }
             if (i == 0 && lane == 0) VW_TRACE(3, globaltimer());
             int valid = 16;
-            if (pg == np - 1) {
-                // a seq_len beyond the table (flagged in the prologue) reads its
-                // pages as full and appends nothing
-                valid = seq_len - pg * 16;
-                const bool in_page = valid <= 16;
-                if (!in_page) valid = 16;
-                if (append && in_page) {
-                    const uint32_t blk = __ldg(p.block_tables + (size_t)b * p.bt_stride + pg);
-                    append_row<T>(p, st, sc, h, blk, valid - 1, lane, nkv);
+            const int lp = WIN ? span.page(pg) : pg;
+            int hide0 = 16, hide1 = 0;               // rows [hide0, hide1) lie outside the window
+            if constexpr (WIN) span.hidden(lp, hide0, hide1);
+            const bool hides = WIN && hide0 < hide1;
+            if (pg == np - 1 || hides) {
+                if (pg == np - 1) {
+                    // a seq_len beyond the table (flagged in the prologue) reads its
+                    // pages as full and appends nothing
+                    valid = seq_len - lp * 16;
+                    const bool in_page = valid <= 16;
+                    if (!in_page) valid = 16;
+                    if (append && in_page) {
+                        const uint32_t blk = __ldg(p.block_tables + (size_t)b * p.bt_stride + lp);
+                        append_row<T>(p, st, sc, h, blk, valid - 1, lane, nkv);
+                    }
+                    if (valid < 16) zero_rows<T>(st, valid, 16, lane);
                 }
-                if (valid < 16) zero_tail<T>(st, valid, lane);
+                if (hides) zero_rows<T>(st, hide0, hide1, lane);
                 // plain stores into a TMA-filled stage: order them before the stage's
                 // next asynchronous (TMA) write, which follows the empty arrive below
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1002,7 +1017,8 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
 
 
             // ---- online softmax (log2 domain) with a lazily raised maximum
-            const bool v0 = t0 < valid, v1 = t1 < valid;
+            const bool v0 = t0 < valid && !(hides && t0 >= hide0 && t0 < hide1);
+            const bool v1 = t1 < valid && !(hides && t1 >= hide0 && t1 < hide1);
             float sv[T::NT][4];
             bool need = false;
 #pragma unroll
@@ -1185,7 +1201,7 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
     if (ctid == 0) VW_TRACE(6, globaltimer());
 }
 
-template <class T>
+template <class T, bool WIN>
 __global__ void __launch_bounds__(T::THREADS, T::MIN_CTAS)
 decode_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -1248,8 +1264,8 @@ decode_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p) {
         }
     } else if (warp == T::W) {
         if (lane == 0) prefetch_tensormap(&tmap);
-        warp_prefixes(p.seq_lens, (int)p.B, (int)p.bt_stride, p.err, blockIdx.x == 0, sm.pfx, sm.nzp,
-                      sm.slen, lane);
+        warp_prefixes<WIN>(p.seq_lens, (int)p.B, (int)p.bt_stride, p.err, blockIdx.x == 0, sm.pfx, sm.nzp,
+                           sm.slen, lane, p.window, p.sinks);
     }
     __syncthreads();
     if (threadIdx.x == 0) VW_TRACE(1, globaltimer());
@@ -1280,14 +1296,14 @@ decode_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p) {
         }
         DecodeParams pp = p;
         if (!early) pp.flags &= ~(kDecodePdl | kDecodeEarlyPages);   // already waited above
-        producer<T>(&tmap, pp, sm, begin, end - begin, first_ord, T::PW == 1 ? 0 : warp - T::W,
+        producer<T, WIN>(&tmap, pp, sm, begin, end - begin, first_ord, T::PW == 1 ? 0 : warp - T::W,
                     deadline);
     } else {
         if (early) {
             griddep_wait();            // q, k_new, v_new may come from the predecessor
             if (threadIdx.x == 0) VW_TRACE(8, globaltimer());
         }
-        consumer<T>(p, sm, begin, end, deadline);
+        consumer<T, WIN>(p, sm, begin, end, deadline);
     }
     if (threadIdx.x == 0) VW_TRACE(7, globaltimer());
 }
@@ -1315,7 +1331,7 @@ constexpr int kCombineMinBlocks = 25;  // 65,536 / (32 x 25) -> a cap of 80 regi
 // Launched as a programmatic dependent of its decode grid: the geometry is
 // computed while the decode still runs, the partials are read after
 // griddepcontrol.wait.  Each thread produces four consecutive output elements.
-template <int D, int G, int IO>
+template <int D, int G, int IO, bool WIN>
 __global__ void __launch_bounds__(kCombineThreads, kCombineMinBlocks) combine_kernel(const DecodeParams p, int dec_grid,
                                                                   float vfold) {
     __shared__ int red[kCombineThreads / 32][4];
@@ -1329,6 +1345,7 @@ __global__ void __launch_bounds__(kCombineThreads, kCombineMinBlocks) combine_ke
     auto pages = [&](int i) {
         const int sl = (int)__ldcg(p.seq_lens + i);
         const int np = (sl + 15) >> 4;
+        if (WIN && sl > 0) return decode_span(sl, (int)p.bt_stride, p.window, p.sinks).n;
         return sl <= 0 ? 0 : min(np, (int)p.bt_stride);
     };
     // pages and sequences with pages, before b and in all (the decode's prefixes)
@@ -1387,7 +1404,7 @@ __global__ void __launch_bounds__(32) plan_kernel(const DecodeParams p, int* pla
     __shared__ int pfx[kMaxBatchPerLaunch + 1], nzp[kMaxBatchPerLaunch + 1];
     const int lane = threadIdx.x;
     const int B = (int)p.B, Hkv = (int)p.Hkv;
-    warp_prefixes(p.seq_lens, B, (int)p.bt_stride, p.err, blockIdx.x == 0, pfx, nzp, nullptr, lane);
+    warp_prefixes<false>(p.seq_lens, B, (int)p.bt_stride, p.err, blockIdx.x == 0, pfx, nzp, nullptr, lane, 0, 0);
     __syncwarp();
     if (blockIdx.x == 0) {
         if (lane == 0) {
@@ -1437,7 +1454,7 @@ cudaError_t launch_decode_plan(const DecodeParams& p, int grid, int* plan, cudaS
 
 namespace {
 
-template <class T>
+template <class T, bool WIN>
 cudaError_t launch_combine(const DecodeLaunch& L) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(L.p.B * L.p.Hkv, (L.p.group + kCombineWarps - 1) / kCombineWarps);
@@ -1448,10 +1465,10 @@ cudaError_t launch_combine(const DecodeLaunch& L) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, combine_kernel<T::D, T::G, T::IO>, L.p, L.grid, T::VFOLD);
+    return cudaLaunchKernelEx(&cfg, combine_kernel<T::D, T::G, T::IO, WIN>, L.p, L.grid, T::VFOLD);
 }
 
-template <class T>
+template <class T, bool WIN>
 cudaError_t launch_t(const DecodeLaunch& L) {
     // the dynamic-smem opt-in is per device; remember it per device ordinal
     static std::atomic<uint64_t> configured{0};
@@ -1459,13 +1476,13 @@ cudaError_t launch_t(const DecodeLaunch& L) {
     cudaGetDevice(&dev);
     const uint64_t bit = 1ull << (dev & 63);
     if (!(configured.load() & bit)) {
-        cudaError_t e = cudaFuncSetAttribute(decode_kernel<T>,
+        cudaError_t e = cudaFuncSetAttribute(decode_kernel<T, WIN>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(decode_kernel<T>, cudaFuncAttributePreferredSharedMemoryCarveout,
+            e = cudaFuncSetAttribute(decode_kernel<T, WIN>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                      (int)cudaSharedmemCarveoutMaxShared);
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(combine_kernel<T::D, T::G, T::IO>,
+            e = cudaFuncSetAttribute(combine_kernel<T::D, T::G, T::IO, WIN>,
                                      cudaFuncAttributePreferredSharedMemoryCarveout,
                                      (int)cudaSharedmemCarveoutMaxShared);
         if (e != cudaSuccess) return e;
@@ -1483,15 +1500,21 @@ cudaError_t launch_t(const DecodeLaunch& L) {
         cfg.attrs = attr;
         cfg.numAttrs = 1;
     }
-    cudaError_t e = cudaLaunchKernelEx(&cfg, decode_kernel<T>, *L.tmap, L.p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, decode_kernel<T, WIN>, *L.tmap, L.p);
     if (e != cudaSuccess) return e;
-    return launch_combine<T>(L);
+    return launch_combine<T, WIN>(L);
 }
 
 template <int D, int KV, int IO>
 cudaError_t launch_d(const DecodeLaunch& L) {
-    if (L.p.group <= 8) return launch_t<Traits<D, 1, KV, IO>>(L);
-    return launch_t<Traits<D, 2, KV, IO>>(L);
+    // the windowed kernels are instances of their own, so that the others keep
+    // the registers and the code that they had
+    if (L.p.window > 0) {
+        if (L.p.group <= 8) return launch_t<Traits<D, 1, KV, IO>, true>(L);
+        return launch_t<Traits<D, 2, KV, IO>, true>(L);
+    }
+    if (L.p.group <= 8) return launch_t<Traits<D, 1, KV, IO>, false>(L);
+    return launch_t<Traits<D, 2, KV, IO>, false>(L);
 }
 
 }  // namespace

@@ -13,6 +13,7 @@ constexpr int kBlockSize = 16;          // tokens per page (engine/engine.bm:102
 constexpr int kMaxBatchPerLaunch = 1024; // sequences per decode launch (prefix tables in smem)
 constexpr int kMinPagesPerCta = 8;      // work quantum when the batch is tiny
 constexpr int kMaxSegmentCost = 64;     // bound of DecodeParams::seg_cost
+constexpr uint32_t kMaxWindow = 1u << 30;   // windows and sinks are clamped to it (positions stay below)
 
 // Everything a decode launch needs besides the tensor map.
 struct DecodeParams {
@@ -34,6 +35,7 @@ struct DecodeParams {
     uint32_t flags;             // kDecodePdl | kDecodeEarlyPages | kDecodePlanned
     uint32_t seg_cost;          // virtual pages per segment boundary in the CTA split (<= kMaxSegmentCost)
     uint64_t wait_cycles;       // bound of the device waits in SM cycles (0: kWaitDeadlineCycles)
+    uint32_t window, sinks;     // window > 0: the mask of PageSpan (both at most kMaxWindow)
 };
 
 constexpr uint32_t kDecodePdl = 0x1u;
@@ -94,6 +96,7 @@ struct PrefillParams {
     // (vw_debug_set_wait_limit) the K/V tiles are withheld, so the first waits
     // are ones that nothing completes and run out
     uint64_t wait_cycles;
+    uint32_t window, sinks;     // window > 0: the mask of PageSpan (both at most kMaxWindow)
 };
 
 struct PrefillLaunch {

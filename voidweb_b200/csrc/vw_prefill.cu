@@ -47,6 +47,7 @@
 #include "vw_ptx.cuh"
 #include "vw_rope.cuh"
 #include "vw_tc.cuh"
+#include "vw_window.cuh"
 
 namespace vw {
 
@@ -279,15 +280,24 @@ struct Fp8RoundRegs {
     float ks, vs;
 };
 
-template <class T>
-__device__ __forceinline__ void fp8_round_ids(const uint32_t* bt, int t, int npages, uint32_t (&blk)[T::R]) {
+template <class T, bool WIN>
+__device__ __forceinline__ void fp8_round_ids(const uint32_t* bt, int t, int npages, const PageSpan& sp,
+                                              uint32_t (&blk)[T::R]) {
 #pragma unroll
-    for (int pg = 0; pg < T::R; ++pg) blk[pg] = t * T::R + pg < npages ? __ldg(bt + t * T::R + pg) : 0xFFFFFFFFu;
+    for (int pg = 0; pg < T::R; ++pg) {
+        const int o = t * T::R + pg;
+        blk[pg] = o < npages ? __ldg(bt + (WIN ? sp.page(o) : o)) : 0xFFFFFFFFu;
+    }
 }
 
-template <class T>
+template <class T, bool WIN>
 __device__ __forceinline__ void fp8_load_round(const PrefillParams& p, const uint32_t (&blk)[T::R], int t, int h,
-                                               int total, int npages, int dt, Fp8RoundRegs& r) {
+                                               int total, int npages, const PageSpan& sp, int dt, Fp8RoundRegs& r) {
+    // row rr of the round's page pg: inside the sequence, and seen by some query of the tile
+    auto inside = [&](int pg, int rr) {
+        const int o = t * T::R + pg, pos = (WIN ? sp.page(o) : o) * kBlockSize + rr;
+        return pos < total && (!WIN || pos < sp.sinks || pos >= sp.lo);
+    };
     if (dt == 0)
 #pragma unroll
         for (int pg = 0; pg < T::R; ++pg)
@@ -299,12 +309,12 @@ __device__ __forceinline__ void fp8_load_round(const PrefillParams& p, const uin
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int pg = (i & 7) >> 1, rr = (i & 1) * 8 + (dt >> 3);
-        const bool valid = blk[pg] < p.num_blocks && t * T::KEYS + pg * 16 + rr < total;
+        const bool valid = blk[pg] < p.num_blocks && inside(pg, rr);
         r.w[i] = valid ? __ldg(reinterpret_cast<const uint4*>(p.kv_data + (head_row(blk[pg], i >> 3) + rr) * T::D + e0))
                        : make_uint4(0, 0, 0, 0);
     }
     const int pg = dt >> 4, rr = dt & 15;
-    const bool valid = blk[pg] < p.num_blocks && t * T::KEYS + dt < total;
+    const bool valid = blk[pg] < p.num_blocks && inside(pg, rr);
     r.ks = valid ? __ldg(p.kv_scales + head_row(blk[pg], 0) + rr) * 256.0f : 0.0f;
     r.vs = valid ? __ldg(p.kv_scales + head_row(blk[pg], 1) + rr) : 0.0f;
 }
@@ -354,7 +364,7 @@ __device__ __forceinline__ void fp8_store_round(uint8_t* kt, uint8_t* vt, float*
 //    S, mask, run the online softmax with a lazily raised maximum (O in tensor
 //    memory is rescaled only when a row's maximum grows by more than 2^8) and
 //    write P over S; finally read O, divide by the row sum and store the rows.
-template <class T>
+template <class T, bool WIN>
 __global__ void __launch_bounds__(T::THREADS, 2)
 prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -441,7 +451,14 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
     const int t0 = (x - tpfx[b]) * kTcRows;
     const int qmax = cs + min(t0 + kTcRows - 1, n - 1);          // last query position of the tile
     const int kend = p.causal ? qmax + 1 : total;                // keys [0, kend)
-    const int npages = (kend + kBlockSize - 1) / kBlockSize;
+    // pages visited; with a window the ones that some query of the tile sees
+    // (ordinals, mapped by span.page)
+    int npages = (kend + kBlockSize - 1) / kBlockSize;
+    PageSpan span{};
+    if constexpr (WIN) {
+        span = page_span(npages, cs + t0, p.window, p.sinks);
+        npages = span.n;
+    }
     const int nrounds = (npages + T::R - 1) / T::R;
     const int j = blockIdx.y, h = j / (int)p.group;
 
@@ -505,15 +522,15 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
         const uint32_t* bt = p.block_tables + (size_t)b * p.bt_stride;
         bool ok = true;
         uint32_t nblk[T::R];
-        fp8_round_ids<T>(bt, 0, npages, nblk);
+        fp8_round_ids<T, WIN>(bt, 0, npages, span, nblk);
         for (int t = 0; t < nrounds && !withhold; ++t) {
             const int st_i = t % T::NST;
             uint32_t blk[T::R];
 #pragma unroll
             for (int pg = 0; pg < T::R; ++pg) blk[pg] = nblk[pg];
             Fp8RoundRegs r;
-            fp8_load_round<T>(p, blk, t, h, total, npages, dt, r);   // in flight during the wait
-            fp8_round_ids<T>(bt, t + 1, npages, nblk);
+            fp8_load_round<T, WIN>(p, blk, t, h, total, npages, span, dt, r);   // in flight during the wait
+            fp8_round_ids<T, WIN>(bt, t + 1, npages, span, nblk);
             // the V tile's release follows the K tile's (P V is committed after S)
             if (t >= T::NST &&
                 !__all_sync(0xffffffffu, mbar_wait(&empty_v[st_i], ((t / T::NST) - 1) & 1, deadline))) {
@@ -542,17 +559,17 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
         uint8_t* tiles = kv ? vtiles : ktiles;
         const uint32_t* bt = p.block_tables + (size_t)b * p.bt_stride;
         if (lane == 0) prefetch_tensormap(&tmap);
-        constexpr int WIN = 32 / T::R;                // rounds per id window
-        uint32_t win = lane < npages ? __ldg(bt + lane) : 0xFFFFFFFFu;
-        uint32_t nwin = 32 + lane < npages ? __ldg(bt + 32 + lane) : 0xFFFFFFFFu;
+        constexpr int IDW = 32 / T::R;                // rounds per window of ids
+        auto id_of = [&](int o) { return o < npages ? __ldg(bt + (WIN ? span.page(o) : o)) : 0xFFFFFFFFu; };
+        uint32_t win = id_of(lane);
+        uint32_t nwin = id_of(32 + lane);
         bool ok = true;
         int issued = 0;
         for (int t = 0; t < nrounds && !withhold; ++t) {
             const int st_i = t % ns;
-            if (t > 0 && t % WIN == 0) {
+            if (t > 0 && t % IDW == 0) {
                 win = nwin;
-                const int pn = (t / WIN + 1) * 32 + lane;
-                nwin = pn < npages ? __ldg(bt + pn) : 0xFFFFFFFFu;
+                nwin = id_of((t / IDW + 1) * 32 + lane);
             }
             if (t >= ns && !__all_sync(0xffffffffu, mbar_wait(&ebar[st_i], ((t / ns) - 1) & 1, deadline))) {
                 ok = false;
@@ -566,7 +583,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
             // (the producers share their schedulers with the softmax warps, so
             // the round's copies go out as one warp instruction)
             const int pg = lane / T::CH, c = lane % T::CH;
-            const uint32_t bj = __shfl_sync(0xffffffffu, win, (t % WIN) * T::R + (pg < T::R ? pg : 0));
+            const uint32_t bj = __shfl_sync(0xffffffffu, win, (t % IDW) * T::R + (pg < T::R ? pg : 0));
             if (pg < m) {
                 int row0 = -32;                          // negative rows: TMA zero-fills
                 if (bj < p.num_blocks)
@@ -610,7 +627,30 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
                 const int bb = t & 1, st_i = t % T::NSTV;
                 if (!mbar_wait(&p_full[bb], (t >> 1) & 1, deadline)) return false;
                 if (!mbar_wait(&full_v[st_i], (t / T::NSTV) & 1, deadline)) return false;
-                const int keyl = total - t * T::KEYS;   // keys of the round inside the sequence
+                const int keyl = WIN ? 0 : total - t * T::KEYS;   // keys of the round inside the sequence
+                if constexpr (WIN && !T::FP8) {
+                    // V rows that no query of the tile sees, outside the window or
+                    // past the sequence's end: zeroed, as below, in the few pages
+                    // that hold some
+                    uint8_t* vt = vtiles + st_i * T::TILE;
+                    bool wrote = false;
+                    for (int pg = 0; pg < T::R && t * T::R + pg < npages; ++pg) {
+                        const int lp = span.page(t * T::R + pg);
+                        int a, z;
+                        span.hidden(lp, a, z);
+                        const int endr = total - lp * kBlockSize;
+                        if (a >= z && endr >= kBlockSize) continue;
+                        wrote = true;
+                        for (int row = 0; row < kBlockSize; ++row) {
+                            if (!(row >= a && row < z) && row < endr) continue;
+                            for (int c = 0; c < T::CH; ++c)
+                                for (int u = 0; u < 8; ++u)
+                                    *reinterpret_cast<uint4*>(vt + c * (T::KEYS * 128) + (pg * kBlockSize + row) * 128 +
+                                                              u * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    if (wrote) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
                 if (!T::FP8 && keyl < T::KEYS && keyl > 0 && (keyl & 15)) {
                     // the page-head holding the sequence's last key: its V rows past
                     // the end hold whatever the pool has there; zero them so that
@@ -665,6 +705,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
         const int r = threadIdx.x, tq = t0 + r;
         const bool live = tq < n;
         const int kend_r = live ? (p.causal ? cs + tq + 1 : total) : 0;
+        const int lo_r = WIN ? max(0, kend_r - (int)p.window) : 0;   // first key of the row's window
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
         float m_ref = -INFINITY, l = 0.0f;
         bool ok = true;
@@ -703,13 +744,25 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
             // folded into the exponent below.
             const int key0 = t * T::KEYS;
             float tmax = -INFINITY;
-            if (__all_sync(0xffffffffu, key0 + T::KEYS <= kend_r)) {
+            bool whole = key0 + T::KEYS <= kend_r;      // the row sees every key of the round
+            if constexpr (WIN) {
+                const int f = span.page(t * T::R) * kBlockSize, e = span.page(t * T::R + T::R - 1) * kBlockSize;
+                // (a round of sink pages and window pages is taken key by key)
+                whole = e - f == (T::R - 1) * kBlockSize && e + kBlockSize <= kend_r &&
+                        (f >= lo_r || e + kBlockSize <= span.sinks);
+            }
+            if (__all_sync(0xffffffffu, whole)) {
 #pragma unroll
                 for (int k = 0; k < T::KEYS; ++k) tmax = fmaxf(tmax, xs[k]);
             } else {
 #pragma unroll
                 for (int k = 0; k < T::KEYS; ++k) {
-                    xs[k] = key0 + k < kend_r ? xs[k] : -INFINITY;
+                    if constexpr (WIN) {
+                        const int pos = span.page(t * T::R + k / kBlockSize) * kBlockSize + k % kBlockSize;
+                        xs[k] = pos < kend_r && (pos >= lo_r || pos < span.sinks) ? xs[k] : -INFINITY;
+                    } else {
+                        xs[k] = key0 + k < kend_r ? xs[k] : -INFINITY;
+                    }
                     tmax = fmaxf(tmax, xs[k]);
                 }
             }
@@ -810,14 +863,18 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
     }
 }
 
-template <class T>
-cudaError_t launch_t(const PrefillLaunch& L) {
-    static std::atomic<bool> configured{false};
-    if (!configured.load()) {
-        cudaError_t e = cudaFuncSetAttribute(prefill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+template <class T, bool WIN>
+cudaError_t launch_w(const PrefillLaunch& L) {
+    // the dynamic-smem opt-in is per device; remember it per device ordinal
+    static std::atomic<uint64_t> configured{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(configured.load() & bit)) {
+        cudaError_t e = cudaFuncSetAttribute(prefill_kernel<T, WIN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              T::SMEM);
         if (e != cudaSuccess) return e;
-        configured.store(true);
+        configured.fetch_or(bit);
     }
     const PrefillParams& p = L.p;
     // an upper bound on the query tiles: sum over b of ceil(n_b / 128) <= T / 128 + B
@@ -834,7 +891,13 @@ cudaError_t launch_t(const PrefillLaunch& L) {
         cfg.attrs = attr;
         cfg.numAttrs = 1;
     }
-    return cudaLaunchKernelEx(&cfg, prefill_kernel<T>, *L.tmap, p);
+    return cudaLaunchKernelEx(&cfg, prefill_kernel<T, WIN>, *L.tmap, p);
+}
+
+// (the windowed kernels are instances of their own, as in the decode)
+template <class T>
+cudaError_t launch_t(const PrefillLaunch& L) {
+    return L.p.window > 0 ? launch_w<T, true>(L) : launch_w<T, false>(L);
 }
 
 }  // namespace

@@ -31,6 +31,15 @@ def _stream(stream=None):
     return ctypes.c_void_p(s.cuda_stream)
 
 
+def _window(window: int, sinks: int):
+    """The C window of (window, sinks); None for (0, 0)."""
+    if window == 0 and sinks == 0:
+        return None
+    if not 0 < window < 1 << 32 or not 0 <= sinks < 1 << 32:
+        raise ValueError(f"window {window} / sinks {sinks}: a window of at least one token, and no fewer than 0 sinks")
+    return C.Window(window, sinks)
+
+
 @dataclass
 class PoolSpec:
     num_layers: int
@@ -121,6 +130,18 @@ class KvPool:
         the default, about 2 s); see vw_debug_set_wait_limit."""
         C.check(C.lib().vw_debug_set_wait_limit(self._h, cycles))
 
+    def _check(self, **tensors) -> None:
+        """Refuse a tensor the kernels would read wrongly: (tensor, shape, element bytes) per name."""
+        for name, (t, shape, size) in tensors.items():
+            if t is None:
+                continue
+            if tuple(t.shape) != shape or t.element_size() != size:
+                raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype}, expected {shape} of {size}-byte elements")
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+            if t.device != self.device:
+                raise ValueError(f"{name} is on {t.device}, the pool on {self.device}")
+
     # -- operations -------------------------------------------------------------
     def append(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor,
                slot_mapping: torch.Tensor, stream=None) -> None:
@@ -132,7 +153,7 @@ class KvPool:
     def paged_decode(self, layer: int, q: torch.Tensor, block_tables: torch.Tensor,
                      seq_lens: torch.Tensor, out: torch.Tensor, k_new=None, v_new=None,
                      scale: float = 0.0, stream=None, flags: int = 0,
-                     rope_theta: float = 0.0) -> torch.Tensor:
+                     rope_theta: float = 0.0, window: int = 0, sinks: int = 0) -> torch.Tensor:
         """o = softmax(q K^T * scale) V over each sequence's pages (GQA, split-K).
 
         With k_new/v_new given, the new token's rows are first written at
@@ -140,21 +161,34 @@ class KvPool:
         [B][stride] int32 ids; seq_lens: [B] int32 (including the new token).
         flags: VW_DECODE_PDL / VW_DECODE_EARLY_PAGES / VW_DECODE_PLANNED (see
         include/voidweb_kv.h).  rope_theta > 0 rotates q and the new K row at
-        position seq_len-1 first (VW_DECODE_ROPE).
+        position seq_len-1 first (VW_DECODE_ROPE).  window > 0: only the last
+        `window` tokens and the first `sinks` tokens are visible (vw_window);
+        block-table entries of pages without a visible token are not read.
         """
         B, Hq, _ = q.shape
+        win = _window(window, sinks)
+        if win is not None:
+            s = self.spec
+            self._check(q=(q, (B, Hq, s.head_dim), 2), out=(out, (B, Hq, s.head_dim), 2),
+                        block_tables=(block_tables, (B, block_tables.shape[-1]), 4), seq_lens=(seq_lens, (B,), 4),
+                        k_new=(k_new, (B, s.num_kv_heads, s.head_dim), 2),
+                        v_new=(v_new, (B, s.num_kv_heads, s.head_dim), 2))
         if rope_theta > 0.0:
             flags |= C.VW_DECODE_ROPE
         a = C.DecodeArgs(layer, B, Hq, block_tables.shape[1], _ptr(q), _ptr(block_tables),
                          _ptr(seq_lens), _ptr(out), _ptr(k_new), _ptr(v_new), scale, flags,
                          rope_theta, 0)
-        C.check(C.lib().vw_paged_decode(self._h, ctypes.byref(a), _stream(stream)))
+        if win is None:
+            C.check(C.lib().vw_paged_decode(self._h, ctypes.byref(a), _stream(stream)))
+        else:
+            C.check(C.lib().vw_paged_decode_window(self._h, ctypes.byref(a), ctypes.byref(win), _stream(stream)))
         return out
 
     def paged_prefill(self, layer: int, q: torch.Tensor, cu_seqlens: torch.Tensor,
                       ctx_start: torch.Tensor, block_tables: torch.Tensor, out: torch.Tensor,
                       k_new=None, v_new=None, causal: bool = True, scale: float = 0.0,
-                      rope_theta: float = 0.0, stream=None, flags: int = 0) -> torch.Tensor:
+                      rope_theta: float = 0.0, stream=None, flags: int = 0, window: int = 0,
+                      sinks: int = 0) -> torch.Tensor:
         """Chunked prefill of one layer (launch_flash_attn_prefill,
         flash_attention.bm:167-177, over the pool's pages).
 
@@ -164,8 +198,18 @@ class KvPool:
         position, else to the whole ctx_start[b] + n_b context.  rope_theta > 0
         rotates q and the appended K rows at their positions (VW_PREFILL_ROPE).
         cu_seqlens, ctx_start: int32; block_tables: [B][stride] int32.
+        window > 0 (causal only): token i sees the last `window` keys up to its
+        own and the first `sinks` keys (vw_window).
         """
         T, Hq, _ = q.shape
+        win = _window(window, sinks)
+        if win is not None:
+            s, B = self.spec, ctx_start.shape[0]
+            self._check(q=(q, (T, Hq, s.head_dim), 2), out=(out, (T, Hq, s.head_dim), 2),
+                        cu_seqlens=(cu_seqlens, (B + 1,), 4), ctx_start=(ctx_start, (B,), 4),
+                        block_tables=(block_tables, (B, block_tables.shape[-1]), 4),
+                        k_new=(k_new, (T, s.num_kv_heads, s.head_dim), 2),
+                        v_new=(v_new, (T, s.num_kv_heads, s.head_dim), 2))
         if causal:
             flags |= C.VW_PREFILL_CAUSAL
         if rope_theta > 0.0:
@@ -173,7 +217,10 @@ class KvPool:
         a = C.PrefillArgs(layer, ctx_start.shape[0], T, Hq, block_tables.shape[1], flags, _ptr(q),
                           _ptr(k_new), _ptr(v_new), _ptr(cu_seqlens), _ptr(ctx_start),
                           _ptr(block_tables), _ptr(out), scale, rope_theta)
-        C.check(C.lib().vw_paged_prefill(self._h, ctypes.byref(a), _stream(stream)))
+        if win is None:
+            C.check(C.lib().vw_paged_prefill(self._h, ctypes.byref(a), _stream(stream)))
+        else:
+            C.check(C.lib().vw_paged_prefill_window(self._h, ctypes.byref(a), ctypes.byref(win), _stream(stream)))
         return out
 
     def plan(self, block_tables: torch.Tensor, seq_lens: torch.Tensor, num_q_heads: int,
@@ -204,12 +251,19 @@ class KvPool:
         return ok, ov, ks, vs
 
     def decode_step_host(self, q, k_new, v_new, block_tables, seq_lens, out,
-                         scale: float = 0.0, stream=None, rope_theta: float = 0.0) -> None:
-        """One step over all layers with host (CPU, ideally pinned) tensors."""
+                         scale: float = 0.0, stream=None, rope_theta: float = 0.0, window: int = 0,
+                         sinks: int = 0) -> None:
+        """One step over all layers with host (CPU, ideally pinned) tensors; window
+        and sinks as in paged_decode, the same for every layer."""
+        win = _window(window, sinks)
         B, Hq = q.shape[1], q.shape[2]
         a = C.StepHostArgs(B, Hq, block_tables.shape[1], 0, _ptr(q), _ptr(k_new), _ptr(v_new),
                            _ptr(block_tables), _ptr(seq_lens), _ptr(out), scale, rope_theta)
-        C.check(C.lib().vw_decode_step_host(self._h, ctypes.byref(a), _stream(stream)))
+        if win is None:
+            C.check(C.lib().vw_decode_step_host(self._h, ctypes.byref(a), _stream(stream)))
+        else:
+            C.check(C.lib().vw_decode_step_host_window(self._h, ctypes.byref(a), ctypes.byref(win),
+                                                       _stream(stream)))
 
 
 def _alias_u8(ptr: int, nbytes: int, device: torch.device) -> torch.Tensor:
