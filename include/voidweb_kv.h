@@ -26,6 +26,14 @@
  *         (kernels/attention/flash_attention.bm:116) stacked over heads,
  *         blocks and layers; one head's K and V page is contiguous
  *   scale [num_layers][num_blocks][num_kv_heads][2][16]  f32, FP8 pools only
+ * 4-bit pools (VW_FP4_E2M1) have no scale buffer:
+ *   data  [num_layers][num_blocks][num_kv_heads] records of 18 * head_dim bytes:
+ *         K codes [16][head_dim/2], V codes [16][head_dim/2] (element 2i in the
+ *         low half of byte i), K scales [16][head_dim/16], V scales
+ *         [head_dim/16][16], the scales E4M3 bytes.  16 consecutive elements of a
+ *         row share the scale s = E4M3(amax / 6); each is the E2M1 code of x / s
+ *         (both to nearest even, saturating; a group whose s rounds to 0 holds
+ *         zeros) and stands for code * s, which f16 and bf16 hold exactly.
  */
 #ifndef VOIDWEB_KV_H
 #define VOIDWEB_KV_H
@@ -53,7 +61,7 @@ typedef enum {
     VW_ERR_DEVICE_CHECK = 5   /* a kernel's bounds check tripped (vw_pool_check) */
 } vw_status;
 
-typedef enum { VW_F16 = 0, VW_BF16 = 1, VW_FP8_E4M3 = 2 } vw_dtype;
+typedef enum { VW_F16 = 0, VW_BF16 = 1, VW_FP8_E4M3 = 2, VW_FP4_E2M1 = 3 } vw_dtype;
 
 /* FP8 codec: the reference's truncating encoder (kernels/norm/rms_norm.bm:98-113)
  * is the default; OCP E4M3FN round-to-nearest-even saturating is optional. */
@@ -75,7 +83,7 @@ typedef struct {
     uint32_t num_blocks;     /* pool size in 16-token blocks, shared by all layers */
     uint32_t kv_dtype;       /* vw_dtype of the pages */
     uint32_t io_dtype;       /* VW_F16 or VW_BF16: q, new K/V rows, outputs; equals
-                                kv_dtype unless the pool is FP8 */
+                                kv_dtype unless the pool is FP8 or 4-bit */
     uint32_t fp8_mode;       /* vw_fp8_mode */
     uint32_t max_batch;      /* most sequences one decode call may carry (<= 1024) */
     int32_t device;          /* CUDA device ordinal */
@@ -99,7 +107,8 @@ VW_API int32_t vw_pool_check(vw_pool* pool, uint32_t* device_error);
 /* Reshape-and-cache (no reference kernel; paging rule of
  * flash_attention.bm:132-140).  k_new, v_new: [num_tokens][num_kv_heads][head_dim]
  * io dtype; slot_mapping: [num_tokens] int64, slot = block*16 + offset, a
- * negative slot skips the token.  FP8 pools quantise each row on the way in. */
+ * negative slot skips the token.  FP8 and 4-bit pools quantise each row on the
+ * way in. */
 VW_API int32_t vw_kv_append(vw_pool* pool, uint32_t layer, const void* k_new, const void* v_new,
                      const int64_t* slot_mapping, uint32_t num_tokens, void* stream);
 
@@ -214,7 +223,8 @@ VW_API int32_t vw_block_copy(vw_pool* pool, const uint32_t* pairs, uint32_t num_
 
 /* Block-table gather of one sequence (paging walk of flash_attention.bm:132-140):
  * raw rows out_k, out_v [num_kv_heads][seq_len][head_dim] in the page element
- * type; FP8 pools also write out_k_scales, out_v_scales [num_kv_heads][seq_len]. */
+ * type; FP8 pools also write out_k_scales, out_v_scales [num_kv_heads][seq_len].
+ * 4-bit pools: the rows' values in the io dtype (exact), no scales. */
 VW_API int32_t vw_kv_gather(vw_pool* pool, uint32_t layer, const uint32_t* block_table,
                      uint32_t seq_len, void* out_k, void* out_v, float* out_k_scales,
                      float* out_v_scales, void* stream);

@@ -49,7 +49,8 @@ def held(x, kv):
         s = (x.abs().amax(-1, keepdim=True) / 448.0).float().double()
         s[s == 0] = 1.0
         return nearest((x / s).float().double(), 4, -6, 448.0) * s
-    g = x.unflatten(-1, (-1, 16))      # "fp4": an E4M3 scale per 16 elements, E2M1 codes
+    # (magnitudes past 6 * 448 saturate alike: cut off before infinities meet frexp)
+    g = x.clamp(-1e6, 1e6).unflatten(-1, (-1, 16))      # "fp4": an E4M3 scale per 16 elements, E2M1 codes
     s = nearest(g.abs().amax(-1, keepdim=True) / 6.0, 4, -6, 448.0)
     return (nearest(g / s.masked_fill(s == 0, math.inf), 2, 0, 6.0) * s).flatten(-2)
 

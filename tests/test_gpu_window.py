@@ -14,7 +14,8 @@ from tests.paged_cases import Batch, attend, check, held, hidden_pages, v_scales
 pytestmark = pytest.mark.gpu
 
 KINDS = [("bf16", "bf16", 128, 28, 4), ("f16", "f16", 64, 14, 2), ("fp8", "bf16", 128, 32, 8), ("fp8", "f16", 128, 24, 2),
-         ("bf16", "bf16", 128, 16, 1), ("bf16", "bf16", 64, 3, 3), ("f16", "f16", 128, 12, 1)]
+         ("bf16", "bf16", 128, 16, 1), ("bf16", "bf16", 64, 3, 3), ("f16", "f16", 128, 12, 1), ("fp4", "bf16", 128, 28, 4),
+         ("fp4", "f16", 64, 14, 2), ("fp4", "f16", 128, 16, 1)]
 WINDOWS = [(1, 0), (1, 1), (16, 0), (17, 3), (100, 4), (33, 16), (64, 40), (5, 1000), (250, 17), (2 ** 32 - 1, 2 ** 32 - 1)]
 LENS = [1, 2, 15, 16, 17, 33, 100, 257, 600, 1000]
 
@@ -51,7 +52,7 @@ def test_decode(kv, io, D, Hq, Hkv, window, sinks):
     check(out, *decode_ref(bt, q, window, sinks), io, kv, f"window {window} sinks {sinks}")
 
 
-@pytest.mark.parametrize("kv,io,D,Hq,Hkv", KINDS[:4])
+@pytest.mark.parametrize("kv,io,D,Hq,Hkv", KINDS[:4] + KINDS[7:9])
 def test_window_of_the_whole_context_is_the_plain_decode(kv, io, D, Hq, Hkv):
     bt = Batch(3, kv, io, D, Hq, Hkv, LENS + [4000]).fill()
     q = bt.rows(bt.B, Hq).to(bt.dev)
@@ -62,7 +63,7 @@ def test_window_of_the_whole_context_is_the_plain_decode(kv, io, D, Hq, Hkv):
     assert torch.equal(a, b)
 
 
-@pytest.mark.parametrize("kv,io,D,Hq,Hkv", [KINDS[0], KINDS[2]])
+@pytest.mark.parametrize("kv,io,D,Hq,Hkv", [KINDS[0], KINDS[2], KINDS[7]])
 def test_decode_split_over_the_grid(kv, io, D, Hq, Hkv):
     """Few long sequences (windows cut across many CTAs) and many short ones."""
     for totals, window, sinks in (([30011, 9000], 8190, 4), ([5000 + 37 * i for i in range(33)], 1000, 20)):
@@ -86,7 +87,7 @@ def device_rope(rows, lens, theta):
     return torch.stack(got)
 
 
-@pytest.mark.parametrize("kv,io,D,Hq,Hkv", [KINDS[0], KINDS[1], KINDS[2]])
+@pytest.mark.parametrize("kv,io,D,Hq,Hkv", [KINDS[0], KINDS[1], KINDS[2], KINDS[7], KINDS[8]])
 def test_fused_append_rope_layers_and_graphs(kv, io, D, Hq, Hkv):
     """The step's rows appended by the decode, with and without rotation, over layers launched as programmatic dependents;
     then captured and replayed.  The rotated step equals the plain step over rows that the library rotated, bit for bit."""
@@ -179,7 +180,7 @@ def test_prefill(kv, io, D, Hq, Hkv, chunks, window, sinks):
         check(out[int(cu[b]):int(cu[b + 1])], *ref, io, kv, f"chunk {b}")
 
 
-@pytest.mark.parametrize("kv,io,D,Hq,Hkv", KINDS[:4])
+@pytest.mark.parametrize("kv,io,D,Hq,Hkv", KINDS[:4] + KINDS[7:9])
 def test_prefill_whole_window_is_the_plain_prefill(kv, io, D, Hq, Hkv):
     bt = Batch(8, kv, io, D, Hq, Hkv, [700, 40]).fill()
     q = bt.rows(340, Hq).to(bt.dev)

@@ -26,7 +26,7 @@ VW_ERR_DEVICE_CHECK = 5
 VW_DEV_ERR_BLOCK_ID, VW_DEV_ERR_SEQ_LEN, VW_DEV_ERR_TIMEOUT, VW_DEV_ERR_SLOT = 0x1, 0x2, 0x4, 0x8
 VW_DEV_ERR_LAUNCH = 0x10
 
-VW_F16, VW_BF16, VW_FP8_E4M3 = 0, 1, 2
+VW_F16, VW_BF16, VW_FP8_E4M3, VW_FP4_E2M1 = 0, 1, 2, 3
 VW_FP8_REFERENCE, VW_FP8_OCP = 0, 1
 VW_DECODE_PDL, VW_DECODE_EARLY_PAGES, VW_DECODE_PLANNED, VW_DECODE_ROPE = 0x1, 0x2, 0x4, 0x8
 VW_PREFILL_CAUSAL, VW_PREFILL_ROPE, VW_PREFILL_PDL = 0x1, 0x2, 0x4

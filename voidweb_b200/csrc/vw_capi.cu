@@ -227,10 +227,10 @@ int32_t vw_pool_create(const vw_pool_config* cfg, vw_pool** out) {
     if (c.reserved != 0) return fail(VW_ERR_INVALID_ARG, "vw_pool_create: reserved must be 0");
     if (c.num_layers == 0 || c.num_kv_heads == 0 || c.num_blocks == 0)
         return fail(VW_ERR_INVALID_ARG, "vw_pool_create: layers, kv heads and blocks must be > 0");
-    if (c.kv_dtype > VW_FP8_E4M3 || (c.io_dtype != VW_F16 && c.io_dtype != VW_BF16))
+    if (c.kv_dtype > VW_FP4_E2M1 || (c.io_dtype != VW_F16 && c.io_dtype != VW_BF16))
         return fail(VW_ERR_INVALID_ARG, "vw_pool_create: bad kv_dtype %u / io_dtype %u",
                     c.kv_dtype, c.io_dtype);
-    if (c.kv_dtype != VW_FP8_E4M3 && c.kv_dtype != c.io_dtype)
+    if (c.kv_dtype < VW_FP8_E4M3 && c.kv_dtype != c.io_dtype)
         return fail(VW_ERR_INVALID_ARG, "vw_pool_create: f16/bf16 pools need io_dtype == kv_dtype");
     if (c.fp8_mode > VW_FP8_OCP) return fail(VW_ERR_INVALID_ARG, "vw_pool_create: bad fp8_mode");
     if (c.head_dim != 64 && c.head_dim != 128)
@@ -256,9 +256,8 @@ int32_t vw_pool_create(const vw_pool_config* cfg, vw_pool** out) {
     p->cfg = c;
     p->geom = PoolGeom{c.num_layers, c.num_kv_heads, c.head_dim, c.num_blocks, c.kv_dtype,
                        c.io_dtype, c.fp8_mode};
-    const uint64_t eb = elem_bytes(c.kv_dtype);
     const uint64_t rows = (uint64_t)c.num_layers * c.num_blocks * 2 * c.num_kv_heads * 16;
-    p->data_bytes = rows * c.head_dim * eb;
+    p->data_bytes = rows / 32 * page_head_bytes(c.kv_dtype, c.head_dim);
     p->scale_bytes = c.kv_dtype == VW_FP8_E4M3 ? rows * 4 : 0;
     cudaError_t e;
     int sms = 0;
@@ -303,7 +302,8 @@ int32_t vw_pool_create(const vw_pool_config* cfg, vw_pool** out) {
         delete p;
         return cuda_fail(e, "vw_pool_create: memset");
     }
-    int32_t rc = encode_pool_map(p);
+    // (4-bit records move as plain bulk copies, without a tensor map)
+    int32_t rc = c.kv_dtype == VW_FP4_E2M1 ? VW_OK : encode_pool_map(p);
     if (rc != VW_OK) {
         pool_free_all(p);
         delete p;

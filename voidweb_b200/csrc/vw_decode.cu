@@ -56,6 +56,7 @@
 #include "vw_fp8.cuh"
 #include "vw_internal.h"
 #include "vw_ptx.cuh"
+#include "vw_fp4.cuh"
 #include "vw_rope.cuh"
 #include "vw_window.cuh"
 
@@ -86,6 +87,16 @@
 #endif
 #ifndef VW_DECODE_FP8_ISSUERS
 #define VW_DECODE_FP8_ISSUERS 1
+#endif
+// 4-bit pages: consumer warps, producer warps, and issuing lanes in each
+#ifndef VW_DECODE_FP4_WARPS
+#define VW_DECODE_FP4_WARPS 4
+#endif
+#ifndef VW_DECODE_FP4_PRODUCERS
+#define VW_DECODE_FP4_PRODUCERS 2
+#endif
+#ifndef VW_DECODE_FP4_ISSUERS
+#define VW_DECODE_FP4_ISSUERS 1
 #endif
 #ifndef VW_DECODE_MAX_STAGES
 #define VW_DECODE_MAX_STAGES 16
@@ -140,22 +151,30 @@ struct Traits {
     static constexpr int D = D_, NT = NT_, KV = KV_, IO = IO_;
     // FP8 pages with one query-head tile: more consumer warps (the E4M3
     // expansion makes the consumers, not the copies, set the pace)
-    static constexpr int W = (KV_ == kFP8 && NT_ == 1) ? kFp8ConsumerWarps : kConsumerWarps;
-    static constexpr int PW = KV_ == kFP8 ? kFp8ProducerWarps : 1;   // producer warps W..W+PW-1
-    static constexpr int IPW = KV_ == kFP8 ? kFp8Issuers : kIssuers;  // issuing lanes per producer warp
+    static constexpr bool FP4 = KV_ == kFP4;
+    // pages read as codes straight into registers, whose fragments leave O^T and
+    // the merge rows in the order of fp8_out_d / fp4_out_d
+    static constexpr bool CODES = KV_ == kFP8 || FP4;
+    static constexpr int W = FP4 ? VW_DECODE_FP4_WARPS
+                                 : (KV_ == kFP8 && NT_ == 1) ? kFp8ConsumerWarps : kConsumerWarps;
+    static constexpr int PW = FP4 ? VW_DECODE_FP4_PRODUCERS
+                                  : KV_ == kFP8 ? kFp8ProducerWarps : 1;   // producer warps W..W+PW-1
+    static constexpr int IPW = FP4 ? VW_DECODE_FP4_ISSUERS
+                                   : KV_ == kFP8 ? kFp8Issuers : kIssuers;  // issuing lanes per producer warp
     static constexpr int NI = PW * IPW;                               // issuers in all
     static constexpr int THREADS = (W + PW) * 32;
     static constexpr int G = 8 * NT;                         // padded query heads per KV head
     static constexpr int EB = KV == kFP8 ? 1 : 2;            // pool element bytes
     static constexpr int ROW = D * EB;                       // bytes of one token row
     static constexpr int CHUNKS = ROW / 128;                 // 128-B swizzle columns per row
-    static constexpr int STAGE = 32 * ROW;                   // one page-head: K rows 0-15, V 16-31
+    // one page-head: K rows 0-15, V 16-31 (4-bit pages: one record)
+    static constexpr int STAGE = FP4 ? Fp4Rec<D>::BYTES : 32 * ROW;
     static constexpr int SCAL = KV == kFP8 ? 128 : 0;        // K and V scales of a page-head
-    static constexpr bool MMA_BF16 = KV == kBF16;            // FP8 pages compute in f16
+    static constexpr bool MMA_BF16 = KV == kBF16;            // FP8 and 4-bit pages compute in f16
     // P as a pair hi + lo of the MMA type, two P V MMAs: a single bf16 (2^-9)
     // or f16 x V-scale (2^-11) probability puts outputs whose few large V terms
     // cancel outside max-abs 2e-3 / rel 1e-2; f16 pools keep a single f16 P
-    static constexpr bool PSPLIT = KV == kBF16 || KV == kFP8;
+    static constexpr bool PSPLIT = KV == kBF16 || CODES;
     // FP8 pages: the V codes are read after the softmax (not with the K codes)
     // when registers are short -- two query-head tiles, or more than four
     // consumer warps -- so that the K and V codes are never live together
@@ -166,7 +185,7 @@ struct Traits {
     // (lanes 4g+c hold query heads 2c, 2c+1, d values 32 apart) then fall on 32
     // different banks.  2-byte pages keep rows of D (a 4-way conflict measured
     // cheaper than the padded rows).
-    static constexpr int MROW = KV == kFP8 ? D + 4 : D;
+    static constexpr int MROW = CODES ? D + 4 : D;
     // the warp states are merged one 8-head tile at a time: [W][8] rows of
     // MROW + 2 floats (o, max, sum), then [W + 2][8] weights, max and sum
     static constexpr int MERGE = W * 8 * (MROW + 2) * 4 + (W + 2) * 8 * 4;
@@ -181,7 +200,7 @@ struct Traits {
                                  align_up_c(QS * QSLOT, 1024) + PFX + PW * 1024 + 1024;
     // resident CTAs per SM the shared memory is sized for: FP8 pages and two
     // query-head tiles need the larger stages and registers of two
-    static constexpr int RES = (NT == 1 && KV != kFP8) ? kCtasPerSm : 2;
+    static constexpr int RES = (NT == 1 && !CODES) ? kCtasPerSm : 2;
     static constexpr int SMEM_CAP = smem_per_cta(RES);
     static constexpr int BUDGET = SMEM_CAP - 1024 /* base alignment slack */ -
                                   (SCAL ? 1024 : 0) /* scale ring alignment */;
@@ -204,13 +223,14 @@ struct Traits {
     // registers (the bound of 3 CTAs' worth of threads), which leaves every SM
     // sub-partition room for the single-warp combine CTAs that wait beside the
     // decode CTAs; the others keep 168 (2 CTAs' worth) to avoid spills.
-    static constexpr int MIN_CTAS = (NT == 1 && KV != kFP8) ? VW_DECODE_MIN_CTAS_2B : 2;
+    static constexpr int MIN_CTAS = (NT == 1 && !CODES) ? VW_DECODE_MIN_CTAS_2B : 2;
     static_assert(CHUNKS >= 1, "row must be at least 128 bytes");
     static_assert(S >= 4, "too few pipeline stages");
     static_assert(S % W == 0 && S % NI == 0, "stage ownership needs S % W == S % issuers == 0");
     static_assert(32 % NI == 0 && IPW <= 32, "issuers must divide the 32-page batch");
     static_assert(SMEM <= SMEM_CAP, "shared memory over the per-CTA limit");
-    static_assert(STAGE % 1024 == 0, "1024-B tile alignment");
+    static_assert(FP4 || STAGE % 1024 == 0, "1024-B tile alignment");
+    static_assert(STAGE % 16 == 0, "bulk copies of whole 16-B units");
 };
 
 // Page as the producer publishes it to its issuing lanes: TMA row of its first
@@ -453,6 +473,19 @@ __device__ void producer(const CUtensorMap* tmap, const DecodeParams& p, const S
         if (ii == 0) VW_TRACE(2, globaltimer());
         if (ii == n - 1) VW_TRACE(4, globaltimer());
         uint8_t* st = sm.stages + s * T::STAGE;
+        if constexpr (T::FP4) {
+            if (pi.row0 >= 0) {
+                mbar_arrive_expect_tx(&sm.full[s], T::STAGE);
+                bulk_load(st, p.kv_data + (size_t)(pi.row0 >> 5) * T::STAGE, T::STAGE, &sm.full[s]);
+            } else {
+                // invalid block id: a record of zeros (as FP8 scales below)
+                for (int k = 0; k < T::STAGE / 16; ++k) reinterpret_cast<uint4*>(st)[k] = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&sm.full[s]);
+            }
+            issued_hi = ii;
+            return true;
+        }
         if constexpr (T::KV == kFP8) {
             float* sc = sm.scal + s * 32;
             if (pi.row0 >= 0) {
@@ -649,24 +682,26 @@ __device__ __forceinline__ void load_q(const DecodeParams& p, const uint8_t* qti
         const int j = nt * 8 + (lane >> 2);
         const bool live = j < (int)p.group;
         const uint8_t* row = qtile + (live ? j : 0) * T::D * 2;
-        if constexpr (T::KV == kFP8) {
+        if constexpr (T::CODES) {
+            // lane c holds elements c*D/4 .. +D/4-1
             const int c = lane & 3;
-            uint32_t w[16];
+            constexpr int NW = T::D / 8;
+            uint32_t w[NW];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const uint4 v = live ? *reinterpret_cast<const uint4*>(row + c * 64 + u * 16)
+            for (int u = 0; u < NW / 4; ++u) {
+                const uint4 v = live ? *reinterpret_cast<const uint4*>(row + c * (T::D / 2) + u * 16)
                                      : make_uint4(0, 0, 0, 0);
                 w[4 * u] = v.x; w[4 * u + 1] = v.y; w[4 * u + 2] = v.z; w[4 * u + 3] = v.w;
             }
             if (p.rope_theta > 0.0f) {
                 const bool lo = c < 2;                  // elements below D/2
 #pragma unroll
-                for (int m = 0; m < 16; ++m) {
+                for (int m = 0; m < NW; ++m) {
                     const uint32_t other = __shfl_xor_sync(0xffffffffu, w[m], 2);
                     const uint32_t rw = lo ? w[m] : other, iw = lo ? other : w[m];
                     float r0 = io_to_f32<T::IO>(rw & 0xFFFFu), i0 = io_to_f32<T::IO>(iw & 0xFFFFu);
                     float r1 = io_to_f32<T::IO>(rw >> 16), i1 = io_to_f32<T::IO>(iw >> 16);
-                    const int d = (c & 1) * 32 + 2 * m;   // index of the lower element
+                    const int d = (c & 1) * (T::D / 4) + 2 * m;   // index of the lower element
                     rope_pair(r0, i0, d, T::D, p.rope_theta, pos);
                     rope_pair(r1, i1, d + 1, T::D, p.rope_theta, pos);
                     w[m] = lo ? ((uint32_t)f32_to_io<T::IO>(r0) | ((uint32_t)f32_to_io<T::IO>(r1) << 16))
@@ -674,15 +709,16 @@ __device__ __forceinline__ void load_q(const DecodeParams& p, const uint8_t* qti
                 }
             }
 #pragma unroll
-            for (int m = 0; m < 16; ++m) {
+            for (int m = 0; m < NW; ++m) {
                 if constexpr (T::IO == kBF16)       // pages compute in f16
                     w[m] = pack2<false>(bf16_bits_to_f32(w[m] & 0xFFFFu), bf16_bits_to_f32(w[m] >> 16));
             }
             // k-step kt: elements 32c+4kt+1, +3 first, then +0, +2 (the K pairs)
 #pragma unroll
             for (int kt = 0; kt < T::KT; ++kt) {
-                qf[nt][kt][0] = __byte_perm(w[2 * kt], w[2 * kt + 1], 0x7632u);
-                qf[nt][kt][1] = __byte_perm(w[2 * kt], w[2 * kt + 1], 0x5410u);
+                // (4-bit pages: the pairs in their own order)
+                qf[nt][kt][0] = T::FP4 ? w[2 * kt] : __byte_perm(w[2 * kt], w[2 * kt + 1], 0x7632u);
+                qf[nt][kt][1] = T::FP4 ? w[2 * kt + 1] : __byte_perm(w[2 * kt], w[2 * kt + 1], 0x5410u);
             }
         } else {
 #pragma unroll
@@ -728,7 +764,16 @@ __device__ __forceinline__ void append_row(const DecodeParams& p, uint8_t* stage
         // pool row of (layer, block, head, kv, t) in [L][NB][Hkv][2][16]
         const size_t prow = ((((size_t)p.layer * p.num_blocks + blk) * p.Hkv + h) * 2 + kv) * 16 + t;
         const int srow = kv * 16 + t;
-        if constexpr (T::KV != kFP8) {
+        if constexpr (T::FP4) {
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < PER / 2; ++k) {
+                v[2 * k] = io_to_f32<T::IO>(nkv[kv][k] & 0xFFFFu);
+                v[2 * k + 1] = io_to_f32<T::IO>(nkv[kv][k] >> 16);
+            }
+            uint8_t* rec = p.kv_data + (((size_t)p.layer * p.num_blocks + blk) * p.Hkv + h) * T::STAGE;
+            fp4_store_row<T::D>(stage, blk_ok ? rec : nullptr, kv, t, lane, v);
+        } else if constexpr (T::KV != kFP8) {
             const uint32_t* w = nkv[kv];
             uint8_t* gdst = p.kv_data + prow * T::ROW + lane * PER * 2;
             uint8_t* sdst = stage + swz16(srow, lane * PER);
@@ -765,6 +810,15 @@ __device__ __forceinline__ void append_row(const DecodeParams& p, uint8_t* stage
 // NaN/Inf through 0 * garbage in the P.V product.
 template <class T>
 __device__ __forceinline__ void zero_rows(uint8_t* stage, int from, int to, int lane) {
+    if constexpr (T::FP4) {
+        using R = Fp4Rec<T::D>;
+        // (codes and scales: a code of 0 times a NaN scale is NaN)
+        for (int k = lane; k < (to - from) * (R::CODE_ROW / 16); k += 32)
+            reinterpret_cast<uint4*>(stage + R::V + from * R::CODE_ROW)[k] = make_uint4(0, 0, 0, 0);
+        for (int k = lane; k < (to - from) * R::GROUPS; k += 32)
+            stage[R::VS + k % R::GROUPS * 16 + from + k / R::GROUPS] = 0;
+        return;
+    }
     const int per_row = T::CHUNKS * 8;                   // 16-B pieces per row
     const int total = (to - from) * per_row;
     for (int k = lane; k < total; k += 32) {
@@ -814,6 +868,72 @@ __device__ __forceinline__ void load_fp8_codes(const uint8_t* st, int lane, int 
     }
 }
 
+// 4-bit page-head fragments (D elements; the record in vw_fp4.cuh).  The A rows of
+// S^T = K Q^T and the columns of V^T are tokens in an order of our choosing,
+// fp4_token(r) = r ^ (r/2 & 1): two rows that lanes of one load phase read then lie an odd
+// number of rows apart, which halves the bank conflicts of the V loads.
+//  * K: lane (g, c) takes the D/4 codes c*D/4 .. of token rows g and g+8; k-step kt uses its
+//    codes 4kt .. 4kt+3 (the reduction order inside a k-step is free), so its
+//    scales are those of one or two groups only.
+//  * V: lane (g, c) takes the D/8 codes g*D/8 .. of token rows 2c, 2c+1, 2c+8, 2c+9; the
+//    codes of two rows interleave into bytes that convert to a pair (two tokens,
+//    one element) at once; row r of d-tile mt is fp4_out_d(r, mt).
+__device__ __forceinline__ int fp4_token(int r) { return r ^ ((r >> 1) & 1); }
+
+template <int D>
+__host__ __device__ __forceinline__ int fp4_out_d(int r, int mt) {
+    return (D / 8) * (r & 7) + (D / 16) * (r >> 3) + mt;
+}
+
+template <int D>
+struct Fp4Codes {
+    uint32_t k[2][D / 32];     // codes of token rows g, g+8
+    uint32_t v[4][D / 64];     // of token rows 2c, 2c+1, 2c+8, 2c+9
+    uint32_t ks[2][D / 64];    // K scales, each twice (f16 pair), of the lane's one or two groups
+    uint32_t vs[2];            // V scales of the token pairs (f16 pairs)
+};
+
+template <int D>
+__device__ __forceinline__ void load_fp4_codes(const uint8_t* st, int lane, Fp4Codes<D>& f) {
+    using R = Fp4Rec<D>;
+    const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int rr = 0; rr < 2; ++rr) {
+        const int tok = fp4_token(g) + 8 * rr;
+        const uint8_t* kp = st + tok * R::CODE_ROW + c * (D / 8);
+        if constexpr (D == 128) {
+            const uint4 w = *reinterpret_cast<const uint4*>(kp);
+            f.k[rr][0] = w.x; f.k[rr][1] = w.y; f.k[rr][2] = w.z; f.k[rr][3] = w.w;
+            const uint32_t s = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(st + R::KS + tok * R::GROUPS + 2 * c));
+            f.ks[rr][0] = __byte_perm(s, s, 0x1010u);
+            f.ks[rr][1] = __byte_perm(s, s, 0x3232u);
+        } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(kp);
+            f.k[rr][0] = w.x; f.k[rr][1] = w.y;
+            const uint32_t s = e4m3x2_to_f16x2(st[R::KS + tok * R::GROUPS + c]);
+            f.ks[rr][0] = __byte_perm(s, s, 0x1010u);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int tok = fp4_token(2 * c + (r & 1)) + 8 * (r >> 1);
+        const uint8_t* vp = st + R::V + tok * R::CODE_ROW + g * (D / 16);
+        if constexpr (D == 128) {
+            const uint2 w = *reinterpret_cast<const uint2*>(vp);
+            f.v[r][0] = w.x; f.v[r][1] = w.y;
+        } else {
+            f.v[r][0] = *reinterpret_cast<const uint32_t*>(vp);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        // tokens 2c, 2c+1 of the group, in the order of the rows above
+        const uint32_t s = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(
+            st + R::VS + (D == 128 ? g : g >> 1) * 16 + 8 * q + 2 * c));
+        f.vs[q] = __byte_perm(s, s, (c & 1) ? 0x1032u : 0x3210u);
+    }
+}
+
 __device__ __forceinline__ uint32_t word_of(const uint4& h, int k) {
     return k == 0 ? h.x : k == 1 ? h.y : k == 2 ? h.z : h.w;
 }
@@ -829,10 +949,11 @@ __host__ __device__ __forceinline__ int fp8_out_d(int r, int mt) {
 // 16 apart in one store (lanes g = 0..7); flipping bits 0-2 of d by bits 4-6
 // spreads them over the banks, and with the rows of D + 4 floats of the four
 // query-head pairs a store's 32 lanes meet 32 different banks (a permutation
-// inside each block of 16).
+// inside each block of 16).  head_dim 64 (4-bit pages): d values 8 apart, bits
+// 0-2 flipped by bits 3-5.
 template <class T>
 __device__ __forceinline__ int merge_col(int d) {
-    return T::KV == kFP8 ? d ^ ((d >> 4) & 7) : d;
+    return T::CODES ? d ^ ((d / (T::D / 8)) & 7) : d;
 }
 
 template <class T, bool WIN>
@@ -850,7 +971,7 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
     const int mi = lane >> 3;
     const int k_tok = (lane & 7) + ((mi & 1) << 3), k_hs = mi >> 1;
     const int v_tok = (lane & 7) + ((mi >> 1) << 3), v_hs = mi & 1;
-    const int t0 = lane >> 2, t1 = t0 + 8;
+    const int t0 = T::FP4 ? fp4_token(lane >> 2) : lane >> 2, t1 = t0 + 8;
 
     bool alive = true;
     int seg_k = 0;
@@ -976,6 +1097,12 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
             float ks0 = 1.0f, ks1 = 1.0f, vs0 = 1.0f, vs1 = 1.0f;
             const uint32_t tbase = smem_u32(st);
             Fp8Codes fc;
+            Fp4Codes<T::D> f4;
+            if constexpr (T::FP4) {
+                load_fp4_codes<T::D>(st, lane, f4);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.empty[s]);
+            }
             if constexpr (T::KV == kFP8) {
                 // this lane's codes and scales are all the page-head it needs:
                 // the stage goes back to the producer before any math, or, with
@@ -999,7 +1126,14 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
 #pragma unroll
             for (int kt = 0; kt < T::KT; ++kt) {
                 uint32_t a0, a1, a2, a3;
-                if constexpr (T::KV == kFP8) {
+                if constexpr (T::FP4) {
+                    uint32_t r0[4], r1[4];
+                    fp4x8_to_f16(f4.k[0][kt >> 1], r0);
+                    fp4x8_to_f16(f4.k[1][kt >> 1], r1);
+                    const int j = 2 * (kt & 1), gi = T::D == 128 ? kt >> 2 : 0;
+                    a0 = f16x2_mul(r0[j], f4.ks[0][gi]); a1 = f16x2_mul(r1[j], f4.ks[1][gi]);
+                    a2 = f16x2_mul(r0[j + 1], f4.ks[0][gi]); a3 = f16x2_mul(r1[j + 1], f4.ks[1][gi]);
+                } else if constexpr (T::KV == kFP8) {
                     const uint32_t w0 = run_word(fc.k[0], kt), w1 = run_word(fc.k[1], kt);
                     a0 = fp8_pair_odd(w0); a1 = fp8_pair_odd(w1);
                     a2 = fp8_pair_even(w0); a3 = fp8_pair_even(w1);
@@ -1090,10 +1224,30 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.empty[s]);
             }
+            uint32_t ve[2][2][T::FP4 ? T::D / 64 : 1];     // interleaved V codes [even, odd][token pair][word]
+            if constexpr (T::FP4) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int k = 0; k < T::D / 64; ++k)
+                        fp4_interleave(f4.v[2 * q][k], f4.v[2 * q + 1][k], ve[0][q][k], ve[1][q][k]);
+            }
 #pragma unroll
             for (int mt = 0; mt < T::MT; ++mt) {
                 uint32_t a0, a1, a2, a3;
-                if constexpr (T::KV == kFP8) {
+                if constexpr (T::FP4) {
+                    // elements mt and MT + mt of the lane's run
+                    uint32_t r[4];
+                    const int x1 = T::MT + mt;
+                    fp4x8_to_f16(ve[mt & 1][0][0], r);
+                    a0 = f16x2_mul(r[mt >> 1 & 3], f4.vs[0]);
+                    fp4x8_to_f16(ve[x1 & 1][0][x1 >> 3], r);
+                    a1 = f16x2_mul(r[(x1 & 7) >> 1], f4.vs[0]);
+                    fp4x8_to_f16(ve[mt & 1][1][0], r);
+                    a2 = f16x2_mul(r[mt >> 1 & 3], f4.vs[1]);
+                    fp4x8_to_f16(ve[x1 & 1][1][x1 >> 3], r);
+                    a3 = f16x2_mul(r[(x1 & 7) >> 1], f4.vs[1]);
+                } else if constexpr (T::KV == kFP8) {
                     // byte mt of unit g: d = 16g + mt (rows g) and 16g + 8 + mt (rows g + 8)
                     const int lo = mt >> 2, hi = 2 + (mt >> 2), j = mt & 3;
                     a0 = fp8_pair_cross(word_of(fc.v[0], lo), word_of(fc.v[1], lo), j);
@@ -1112,7 +1266,7 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
                 }
             }
             __syncwarp();
-            if constexpr (T::KV != kFP8) {
+            if constexpr (!T::CODES) {
                 if (lane == 0) mbar_arrive(&sm.empty[s]);
             }
         }
@@ -1141,8 +1295,9 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
 #pragma unroll
             for (int mt = 0; mt < T::MT; ++mt) {
                 // O^T rows lane/4 and lane/4 + 8 of d-tile mt
-                const int dA = T::KV == kFP8 ? fp8_out_d(lane >> 2, mt) : mt * 16 + (lane >> 2);
-                const int dB = T::KV == kFP8 ? fp8_out_d((lane >> 2) + 8, mt) : dA + 8;
+                const int r0 = lane >> 2;
+                const int dA = T::FP4 ? fp4_out_d<T::D>(r0, mt) : T::KV == kFP8 ? fp8_out_d(r0, mt) : mt * 16 + r0;
+                const int dB = T::FP4 ? fp4_out_d<T::D>(r0 + 8, mt) : T::KV == kFP8 ? fp8_out_d(r0 + 8, mt) : dA + 8;
                 mo[jl * T::MROW + merge_col<T>(dA)] = o[nt][mt][0];
                 mo[(jl + 1) * T::MROW + merge_col<T>(dA)] = o[nt][mt][1];
                 mo[jl * T::MROW + merge_col<T>(dB)] = o[nt][mt][2];
@@ -1252,7 +1407,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p) {
         }
         if (warp >= T::W) {
             // every producer warp takes the first batch into its own buffer
-            if (lane == 0) prefetch_tensormap(&tmap);
+            if (!T::FP4 && lane == 0) prefetch_tensormap(&tmap);
             if (warp == T::W && lane < 3) sm.flag[2 + lane] = __ldcg(entry + lane);
             const int4 rec = __ldcg(reinterpret_cast<const int4*>(entry + 4) + lane);
             PageInfo pi;
@@ -1263,7 +1418,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p) {
             sm.pinfo[(warp - T::W) * 64 + lane] = pi;
         }
     } else if (warp == T::W) {
-        if (lane == 0) prefetch_tensormap(&tmap);
+        if (!T::FP4 && lane == 0) prefetch_tensormap(&tmap);
         warp_prefixes<WIN>(p.seq_lens, (int)p.B, (int)p.bt_stride, p.err, blockIdx.x == 0, sm.pfx, sm.nzp,
                            sm.slen, lane, p.window, p.sinks);
     }
@@ -1538,6 +1693,10 @@ extern "C" __attribute__((visibility("default"))) int vw_debug_trace(void* host,
 
 cudaError_t launch_paged_decode(const DecodeLaunch& L) {
     const uint32_t D = L.head_dim;
+    if (L.kv_kind == kFP4) {
+        if (D == 64) return L.io_kind == kBF16 ? launch_d<64, kFP4, kBF16>(L) : launch_d<64, kFP4, kF16>(L);
+        return L.io_kind == kBF16 ? launch_d<128, kFP4, kBF16>(L) : launch_d<128, kFP4, kF16>(L);
+    }
     if (L.kv_kind == kFP8) {
         if (D != 128) return cudaErrorInvalidValue;
         return L.io_kind == kBF16 ? launch_d<128, kFP8, kBF16>(L) : launch_d<128, kFP8, kF16>(L);

@@ -1,0 +1,120 @@
+// vw_fp4.cuh -- 4-bit KV codec on the device and the record it is stored in.
+//
+// Every 16 consecutive elements of a row share the scale s = E4M3(amax / 6) (to
+// nearest even, saturating at 448) and each is held as the E2M1 code of x / s
+// (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives; to nearest even, saturating); a
+// group whose scale rounds to 0 holds zeros.  A code stands for code * s: two
+// times four significant bits between 2^-10 and 2688, exact in f16 and in bf16,
+// so the attention multiplies codes by scales in f16 and rounds nothing.  Both
+// quotients are IEEE f32 divisions; the borders between codes are products of
+// few bits, so they fall on the side the real quotient falls on.  NaN elements
+// encode as 6 (the conversion's rule) and do not count in amax.
+//
+// One page-head (16 tokens of one KV head) is one record of 18 D bytes, which one
+// bulk copy moves:
+//   K codes [16][D/2], V codes [16][D/2]   element 2i in the low half of byte i
+//   K scales [16][D/16]                    a token's groups together
+//   V scales [D/16][16]                    a group's tokens together: the P V product
+//                                          pairs two tokens of one element
+#pragma once
+#include <cstdint>
+
+namespace vw {
+
+template <int D>
+struct Fp4Rec {
+    static constexpr int CODE_ROW = D / 2;      // bytes of one token's codes
+    static constexpr int GROUPS = D / 16;
+    static constexpr int V = 16 * CODE_ROW;     // first V code
+    static constexpr int KS = 2 * V;            // first K scale
+    static constexpr int VS = KS + 16 * GROUPS; // first V scale
+    static constexpr int BYTES = VS + 16 * GROUPS;
+};
+static_assert(Fp4Rec<128>::BYTES == 2304 && Fp4Rec<64>::BYTES == 1152, "18 D bytes");
+
+// E4M3 scale code of a group with the given largest magnitude.
+__device__ __forceinline__ uint32_t fp4_scale_code(float amax) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.0f), "f"(__fdiv_rn(amax, 6.0f)));
+    return r & 0xFFu;
+}
+
+// Two E4M3 codes (low byte first) -> f16 pair.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t codes) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)codes));
+    return r;
+}
+
+__device__ __forceinline__ float e4m3_to_f32(uint32_t code) {
+    return f16_bits_to_f32(e4m3x2_to_f16x2(code) & 0xFFFFu);
+}
+
+// Four elements -> four E2M1 codes, the first in the low half of the low byte.
+__device__ __forceinline__ uint32_t fp4_encode4(const float (&v)[4], uint32_t scale_code) {
+    const float s = e4m3_to_f32(scale_code);
+    if (s == 0.0f) return 0u;
+    const float a = __fdiv_rn(v[0], s), b = __fdiv_rn(v[1], s), c = __fdiv_rn(v[2], s), d = __fdiv_rn(v[3], s);
+    uint16_t r;
+    asm("{\n\t.reg .b8 lo, hi;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 lo, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 hi, %4, %3;\n\t"
+        "mov.b16 %0, {lo, hi};\n\t}"
+        : "=h"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
+    return r;
+}
+
+// Eight codes of a word -> four f16 pairs (exact).  The word is one that its lane
+// loaded whole, or a bitwise mix of such words: ptxas 12.9 turned the byte
+// conversions of a kernel parameter (a uniform register) into an instruction that
+// raised "misaligned address", and those of a zero-extended 16-bit value into zeros.
+__device__ __forceinline__ void fp4x8_to_f16(uint32_t w, uint32_t (&r)[4]) {
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "mov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(w));
+}
+
+// The codes of two words interleaved: even elements into e, odd ones into o, each
+// byte holding a's code in its low half and b's in its high half.
+__device__ __forceinline__ void fp4_interleave(uint32_t a, uint32_t b, uint32_t& e, uint32_t& o) {
+    e = (a & 0x0F0F0F0Fu) | ((b << 4) & 0xF0F0F0F0u);
+    o = ((a >> 4) & 0x0F0F0F0Fu) | (b & 0xF0F0F0F0u);
+}
+
+__device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// One row of a record by one warp: lane l holds elements l*D/32 .. +D/32-1 (the
+// first D/32 of v).  Writes codes and scales of token t into the records at rec
+// and, when rec2 is given, the same at rec2.
+template <int D>
+__device__ __forceinline__ void fp4_store_row(uint8_t* rec, uint8_t* rec2, int kv, int t, int lane, const float (&v)[4]) {
+    using R = Fp4Rec<D>;
+    constexpr int PER = D / 32, LANES = 16 / PER;      // lanes of a group: 4 (D 128) or 8 (D 64)
+    float amax = fmaxf(fabsf(v[0]), fabsf(v[1]));
+    if constexpr (PER == 4) amax = fmaxf(amax, fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+    for (int off = 1; off < LANES; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+    const uint32_t sc = fp4_scale_code(amax);
+    const uint32_t codes = fp4_encode4(v, sc);
+    const int co = kv * R::V + t * R::CODE_ROW + lane * (PER / 2);
+    const int g = lane / LANES;
+    const int so = kv == 0 ? R::KS + t * R::GROUPS + g : R::VS + g * 16 + t;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        uint8_t* r = k == 0 ? rec : rec2;
+        if (!r) continue;
+        if constexpr (PER == 4) *reinterpret_cast<uint16_t*>(r + co) = (uint16_t)codes;
+        else r[co] = (uint8_t)codes;
+        if (lane % LANES == 0) r[so] = (uint8_t)sc;
+    }
+}
+
+}  // namespace vw

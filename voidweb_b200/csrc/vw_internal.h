@@ -7,7 +7,7 @@
 
 namespace vw {
 
-enum KvKind : uint32_t { kF16 = 0, kBF16 = 1, kFP8 = 2 };
+enum KvKind : uint32_t { kF16 = 0, kBF16 = 1, kFP8 = 2, kFP4 = 3 };
 
 constexpr int kBlockSize = 16;          // tokens per page (engine/engine.bm:102)
 constexpr int kMaxBatchPerLaunch = 1024; // sequences per decode launch (prefix tables in smem)
@@ -138,9 +138,19 @@ cudaError_t launch_kv_gather(const PoolGeom& g, const uint8_t* data, const float
                              void* out_k, void* out_v, float* out_ks, float* out_vs,
                              uint32_t* err, cudaStream_t s);
 
+// Bytes of one element of a page; 4-bit pools have records instead (vw_fp4.cuh).
 #ifdef __CUDACC__
 __host__ __device__
 #endif
 inline size_t elem_bytes(uint32_t kv_kind) { return kv_kind == kFP8 ? 1 : 2; }
+
+// Bytes of one page-head: 16 K rows and 16 V rows of one KV head (FP8 scales not
+// counted; a 4-bit record holds its scales).
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+inline uint32_t page_head_bytes(uint32_t kv_kind, uint32_t head_dim) {
+    return kv_kind == kFP4 ? 18u * head_dim : 32u * head_dim * (uint32_t)elem_bytes(kv_kind);
+}
 
 }  // namespace vw

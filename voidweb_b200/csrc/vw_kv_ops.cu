@@ -6,6 +6,7 @@
 // sectors, and keeps several rows' loads in flight before it stores them.  Pool layout:
 //   data  [L][NB][Hkv][2][16][D]   (2 = K, V; element f16/bf16 or an E4M3 code)
 //   scale [L][NB][Hkv][2][16]      (FP8 pools only)
+// or, 4-bit pools, [L][NB][Hkv] records of codes and scales (vw_fp4.cuh).
 // Bounds: every block id and slot is checked against the pool before it is
 // used; a bad one sets a bit in the pool's device error word and the row is
 // skipped, so no kernel here can write outside the pool.
@@ -15,6 +16,7 @@
 #include "vw_fp8.cuh"
 #include "vw_internal.h"
 #include "vw_ptx.cuh"
+#include "vw_fp4.cuh"
 
 namespace vw {
 
@@ -44,6 +46,40 @@ __device__ __forceinline__ uint64_t pool_row(const PoolGeom& g, uint32_t layer, 
 
 constexpr uint32_t kRowsPerWarp = 4;     // a warp's loads of 4 rows are in flight together
 
+// 4-bit record of (layer, block, head).
+template <int D>
+__device__ __forceinline__ uint64_t fp4_record(const PoolGeom& g, uint32_t layer, uint32_t blk, uint32_t h) {
+    return (((uint64_t)layer * g.num_blocks + blk) * g.num_kv_heads + h) * Fp4Rec<D>::BYTES;
+}
+
+// The 4-bit pools' part of the append: rows w0 .. w0+3 of the launch, one row at a time.
+template <int D>
+__device__ __forceinline__ void fp4_append(const PoolGeom& g, uint8_t* data, uint32_t layer, const uint16_t* k_new,
+                                           const uint16_t* v_new, const int64_t* slots, uint32_t w0, uint32_t rows,
+                                           uint32_t lane, uint32_t* err) {
+    for (uint32_t r = 0; r < kRowsPerWarp; ++r) {
+        const uint32_t w = w0 + r;
+        if (w >= rows) return;
+        const RowIdx x = row_index(w, g.num_kv_heads);
+        const int64_t slot = __ldg(slots + x.i);
+        if (slot < 0) continue;
+        if (slot >= (int64_t)g.num_blocks * kBlockSize) {
+            if (lane == 0) atomicOr(err, kDevErrSlot);
+            continue;
+        }
+        const uint16_t* src = (x.kv == 0 ? k_new : v_new) + ((size_t)x.i * g.num_kv_heads + x.h) * D + lane * (D / 32);
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) {
+            const uint32_t two = __ldg(reinterpret_cast<const uint32_t*>(src) + k);
+            v[2 * k] = io_f32(two & 0xFFFFu, g.io_kind);
+            v[2 * k + 1] = io_f32(two >> 16, g.io_kind);
+        }
+        fp4_store_row<D>(data + fp4_record<D>(g, layer, (uint32_t)(slot / kBlockSize), x.h), nullptr, (int)x.kv,
+                         (int)(slot % kBlockSize), (int)lane, v);
+    }
+}
+
 // Reshape-and-cache.  The reference has no append kernel; its paging rule
 // (kernels/attention/flash_attention.bm:132-140: token p lives in logical block
 // p/16 at slot p%16) defines slot = block_table[p/16]*16 + p%16.  Warp w of the
@@ -60,6 +96,11 @@ __global__ void __launch_bounds__(256) kv_append_kernel(PoolGeom g, uint8_t* __r
     const uint32_t w0 = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kRowsPerWarp;
     const uint32_t rows = n * 2u * g.num_kv_heads;
     const uint32_t D = g.head_dim;
+    if (g.kv_kind == kFP4) {
+        if (D == 128) fp4_append<128>(g, data, layer, k_new, v_new, slots, w0, rows, lane, err);
+        else fp4_append<64>(g, data, layer, k_new, v_new, slots, w0, rows, lane, err);
+        return;
+    }
     if (g.kv_kind != kFP8) {
         // D 16-bit elements = D/4 u64 words per row: one word per lane (D 128) or
         // one per lane of the first half-warp (D 64)
@@ -135,7 +176,7 @@ __global__ void __launch_bounds__(256) block_copy_kernel(PoolGeom g, uint8_t* __
         if (threadIdx.x == 0) atomicOr(err, kDevErrBlockId);
         return;
     }
-    const uint32_t bytes = 2u * g.num_kv_heads * kBlockSize * g.head_dim * (uint32_t)elem_bytes(g.kv_kind);
+    const uint32_t bytes = g.num_kv_heads * page_head_bytes(g.kv_kind, g.head_dim);
     const uint4* s = reinterpret_cast<const uint4*>(data + ((uint64_t)layer * g.num_blocks + src) * bytes);
     uint4* d = reinterpret_cast<uint4*>(data + ((uint64_t)layer * g.num_blocks + dst) * bytes);
     const uint32_t n16 = bytes / 16;
@@ -157,6 +198,55 @@ __global__ void __launch_bounds__(256) block_copy_kernel(PoolGeom g, uint8_t* __
         const float* ss = scales + ((uint64_t)layer * g.num_blocks + src) * ns;
         float* ds = scales + ((uint64_t)layer * g.num_blocks + dst) * ns;
         for (uint32_t k = threadIdx.x; k < ns; k += blockDim.x) ds[k] = __ldg(ss + k);
+    }
+}
+
+// Block-table gather of a 4-bit pool: the rows' values (exact) in the io type,
+// into [Hkv][seq_len][D].  A warp takes kFp4GatherRows rows; a lane expands a word
+// of eight codes, half a group, into 16 B, so D/8 lanes write a row.
+constexpr uint32_t kFp4GatherRows = 8;
+
+template <int D>
+__global__ void __launch_bounds__(256) fp4_gather_kernel(PoolGeom g, const uint8_t* __restrict__ data, uint32_t layer,
+                                                         const uint32_t* __restrict__ block_table, uint32_t seq_len,
+                                                         uint16_t* __restrict__ out_k, uint16_t* __restrict__ out_v,
+                                                         uint32_t* err) {
+    using R = Fp4Rec<D>;
+    constexpr int WORDS = D / 8, N = kFp4GatherRows * WORDS / 32;      // words of a row, words of a lane
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t w0 = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kFp4GatherRows;
+    const uint32_t rows = seq_len * 2u * g.num_kv_heads;
+    uint32_t code[N], sc[N];
+    uint16_t* dst[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        dst[j] = nullptr;
+        const uint32_t unit = j * 32 + lane, w = w0 + unit / WORDS, word = unit % WORDS;
+        if (w >= rows) continue;
+        const RowIdx x = row_index(w, g.num_kv_heads);      // x.i = the position p
+        const uint32_t blk = __ldg(block_table + x.i / kBlockSize);
+        if (blk >= g.num_blocks) {
+            if (word == 0) atomicOr(err, kDevErrBlockId);
+            continue;
+        }
+        const uint8_t* rec = data + fp4_record<D>(g, layer, blk, x.h);
+        const uint32_t t = x.i % kBlockSize, grp = word / 2;
+        code[j] = __ldg(reinterpret_cast<const uint32_t*>(rec + x.kv * R::V + t * R::CODE_ROW) + word);
+        sc[j] = __ldg(rec + (x.kv == 0 ? R::KS + t * R::GROUPS + grp : R::VS + grp * 16 + t));
+        dst[j] = (x.kv == 0 ? out_k : out_v) + ((size_t)x.h * seq_len + x.i) * D + word * 8;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        if (!dst[j]) continue;
+        uint32_t h[4];
+        fp4x8_to_f16(code[j], h);
+        const uint32_t s2 = e4m3x2_to_f16x2(sc[j] | (sc[j] << 8));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            h[k] = f16x2_mul(h[k], s2);
+            if (g.io_kind == kBF16) h[k] = pack2<true>(f16_bits_to_f32(h[k] & 0xFFFFu), f16_bits_to_f32(h[k] >> 16));
+        }
+        *reinterpret_cast<uint4*>(dst[j]) = make_uint4(h[0], h[1], h[2], h[3]);
     }
 }
 
@@ -231,6 +321,13 @@ cudaError_t launch_kv_gather(const PoolGeom& g, const uint8_t* data, const float
     if (seq_len == 0) return cudaSuccess;
     const uint64_t rows = (uint64_t)seq_len * 2 * g.num_kv_heads;
     const unsigned grid = (unsigned)((rows + 8 * kRowsPerWarp - 1) / (8 * kRowsPerWarp));
+    if (g.kv_kind == kFP4) {
+        const unsigned grid = (unsigned)((rows + 8 * kFp4GatherRows - 1) / (8 * kFp4GatherRows));
+        uint16_t *k = static_cast<uint16_t*>(out_k), *v = static_cast<uint16_t*>(out_v);
+        if (g.head_dim == 128) fp4_gather_kernel<128><<<grid, 256, 0, s>>>(g, data, layer, block_table, seq_len, k, v, err);
+        else fp4_gather_kernel<64><<<grid, 256, 0, s>>>(g, data, layer, block_table, seq_len, k, v, err);
+        return cudaGetLastError();
+    }
     kv_gather_kernel<<<grid, 256, 0, s>>>(g, data, scales, layer, block_table, seq_len,
                                           static_cast<uint8_t*>(out_k), static_cast<uint8_t*>(out_v),
                                           out_ks, out_vs, err);

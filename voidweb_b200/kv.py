@@ -46,7 +46,7 @@ class PoolSpec:
     num_kv_heads: int
     head_dim: int
     num_blocks: int
-    kv_dtype: str = "bf16"      # "f16" | "bf16" | "fp8"
+    kv_dtype: str = "bf16"      # "f16" | "bf16" | "fp8" | "fp4"
     io_dtype: str = "bf16"      # "f16" | "bf16"
     fp8_mode: str = "reference"  # "reference" (reference encoder) | "ocp"
     max_batch: int = 256
@@ -54,16 +54,19 @@ class PoolSpec:
     @property
     def block_bytes(self) -> int:
         """Bytes one block id addresses across all layers (engine/engine.bm:170-182)."""
+        if self.kv_dtype == "fp4":
+            return self.num_layers * self.num_kv_heads * 18 * self.head_dim
         eb = 1 if self.kv_dtype == "fp8" else 2
         s = 4 if self.kv_dtype == "fp8" else 0
         return self.num_layers * 2 * self.num_kv_heads * 16 * (self.head_dim * eb + s)
 
 
-_DT = {"f16": C.VW_F16, "bf16": C.VW_BF16, "fp8": C.VW_FP8_E4M3}
+_DT = {"f16": C.VW_F16, "bf16": C.VW_BF16, "fp8": C.VW_FP8_E4M3, "fp4": C.VW_FP4_E2M1}
 
 
 class KvPool:
-    """A paged KV pool on one GPU: pages [L][NB][Hkv][2][16][D] (+ FP8 scales)."""
+    """A paged KV pool on one GPU: pages [L][NB][Hkv][2][16][D] (+ FP8 scales), or
+    4-bit records [L][NB][Hkv][18 D bytes] (include/voidweb_kv.h)."""
 
     def __init__(self, spec: PoolSpec, device: int | torch.device = 0,
                  data: torch.Tensor | None = None, scales: torch.Tensor | None = None):
@@ -105,6 +108,8 @@ class KvPool:
     @property
     def page_shape(self):
         s = self.spec
+        if s.kv_dtype == "fp4":
+            return (s.num_layers, s.num_blocks, s.num_kv_heads, 18 * s.head_dim)
         return (s.num_layers, s.num_blocks, s.num_kv_heads, 2, 16, s.head_dim)
 
     # -- views of the library-owned pages (for tests and inspection) ----------
@@ -147,6 +152,9 @@ class KvPool:
                slot_mapping: torch.Tensor, stream=None) -> None:
         """Reshape-and-cache: k_new/v_new [n][Hkv][D]; slot = block*16 + offset."""
         n = k_new.shape[0]
+        if self.spec.kv_dtype == "fp4":
+            row = (n, self.spec.num_kv_heads, self.spec.head_dim)
+            self._check(k_new=(k_new, row, 2), v_new=(v_new, row, 2), slot_mapping=(slot_mapping, (n,), 8))
         C.check(C.lib().vw_kv_append(self._h, layer, _ptr(k_new), _ptr(v_new),
                                      _ptr(slot_mapping), n, _stream(stream)))
 
@@ -167,7 +175,7 @@ class KvPool:
         """
         B, Hq, _ = q.shape
         win = _window(window, sinks)
-        if win is not None:
+        if win is not None or self.spec.kv_dtype == "fp4":
             s = self.spec
             self._check(q=(q, (B, Hq, s.head_dim), 2), out=(out, (B, Hq, s.head_dim), 2),
                         block_tables=(block_tables, (B, block_tables.shape[-1]), 4), seq_lens=(seq_lens, (B,), 4),
@@ -203,7 +211,7 @@ class KvPool:
         """
         T, Hq, _ = q.shape
         win = _window(window, sinks)
-        if win is not None:
+        if win is not None or self.spec.kv_dtype == "fp4":
             s, B = self.spec, ctx_start.shape[0]
             self._check(q=(q, (T, Hq, s.head_dim), 2), out=(out, (T, Hq, s.head_dim), 2),
                         cu_seqlens=(cu_seqlens, (B + 1,), 4), ctx_start=(ctx_start, (B,), 4),
@@ -237,9 +245,15 @@ class KvPool:
         C.check(C.lib().vw_block_copy(self._h, _ptr(pairs), pairs.shape[0], _stream(stream)))
 
     def gather(self, layer: int, block_table: torch.Tensor, seq_len: int, stream=None):
-        """Raw K/V rows of one sequence, [Hkv][seq_len][D] (+ FP8 scales)."""
+        """Raw K/V rows of one sequence, [Hkv][seq_len][D] (+ FP8 scales); 4-bit
+        pools: their values in the io dtype."""
         s = self.spec
         dt = torch.uint8 if s.kv_dtype == "fp8" else torch.int16
+        if s.kv_dtype == "fp4":
+            dt = torch.bfloat16 if s.io_dtype == "bf16" else torch.float16
+            if block_table.dim() != 1 or block_table.shape[0] * 16 < seq_len:
+                raise ValueError(f"block_table: {tuple(block_table.shape)} for {seq_len} tokens")
+            self._check(block_table=(block_table, tuple(block_table.shape), 4))
         ok = torch.empty((s.num_kv_heads, seq_len, s.head_dim), dtype=dt, device=self.device)
         ov = torch.empty_like(ok)
         ks = vs = None
