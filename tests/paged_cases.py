@@ -12,7 +12,7 @@ Tolerance of an output with reference r, A = sum p |v| and F (below):
     u * |r| + c * A + 2^-25 * F
 u: half a step of the io type (bf16 2^-8, fp16 2^-11), taken 1% larger for the
 second-order term.  c: probabilities enter the P V product as a pair hi + lo (bf16
-pages 2^-16, FP8 and 4-bit pages 2^-22) or, on f16 pages, as one f16 (2^-11); the
+pages 2^-16, FP8 pages 2^-22) or, on f16 pages and in the decode of 4-bit ones, as one f16 (2^-11); the
 f32 score of up to 128 products of about 2^5 in magnitude (128 * 2^-24 * 2^5 * ln 2
 relative in p: 2^-12.5 at the very worst, rounding errors of both signs and far
 fewer than 128 of them at that size: 2^-14) and ex2.approx (2^-22) add to it.  So
@@ -88,7 +88,7 @@ def check(got, ref, A, F, io, kv, what=""):
     got = got.detach().cpu().double()
     assert torch.isfinite(got).all(), f"{what}: not finite"
     u = torch.finfo(TYPES[io]).eps / 2 * 1.01
-    c = 2.0 ** -13 + (2.0 ** -11 if kv == "f16" else 0.0)
+    c = 2.0 ** -13 + (2.0 ** -11 if kv in ("f16", "fp4") else 0.0)
     tol = u * ref.abs() + c * A + (0.0 if kv == "bf16" else 2.0 ** -25 * F) + 2.0 ** -25
     worst = ((got - ref).abs() / tol).max().item()
     assert worst <= 1.0, f"{what}: {worst:.3g} times the tolerance"

@@ -56,9 +56,7 @@
 #include "vw_fp8.cuh"
 #include "vw_internal.h"
 #include "vw_ptx.cuh"
-#include "vw_fp4.cuh"
 #include "vw_rope.cuh"
-#include "vw_window.cuh"
 
 #ifndef VW_DECODE_WARPS
 #define VW_DECODE_WARPS 4
@@ -88,16 +86,6 @@
 #ifndef VW_DECODE_FP8_ISSUERS
 #define VW_DECODE_FP8_ISSUERS 1
 #endif
-// 4-bit pages: consumer warps, producer warps, and issuing lanes in each
-#ifndef VW_DECODE_FP4_WARPS
-#define VW_DECODE_FP4_WARPS 4
-#endif
-#ifndef VW_DECODE_FP4_PRODUCERS
-#define VW_DECODE_FP4_PRODUCERS 2
-#endif
-#ifndef VW_DECODE_FP4_ISSUERS
-#define VW_DECODE_FP4_ISSUERS 1
-#endif
 #ifndef VW_DECODE_MAX_STAGES
 #define VW_DECODE_MAX_STAGES 16
 #endif
@@ -119,6 +107,12 @@ __device__ unsigned long long g_vw_trace[2 * 1024 * 16];
 #define VW_TRACE(slot, val) ((void)0)
 #endif
 
+}  // namespace vw
+
+#include "vw_split.cuh"
+
+namespace vw {
+
 namespace {
 
 constexpr int kConsumerWarps = VW_DECODE_WARPS;
@@ -137,44 +131,33 @@ __host__ __device__ constexpr int smem_per_cta(int ctas) { return 233472 / ctas 
 // 2-byte pages feed ldmatrix in place from the stage, [CHUNKS][32 rows][128 B]
 // (column stride 4096 B); FP8 pages are read as codes straight into registers
 constexpr int kStageColumn = 4096;
-constexpr float kRescaleThreshold = 8.0f;             // log2 units: p <= 2^8 vs a stale max
 
 // E4M3 codes -> f16 pairs for the MMA fragments hold value / 256; the 256 is
 // folded into the K scales and the output.
 constexpr float kFp8Fold = 256.0f;
 
-__host__ __device__ constexpr int align_up_c(int x, int a) { return (x + a - 1) / a * a; }
-__host__ __device__ constexpr int gcd_c(int a, int b) { return b == 0 ? a : gcd_c(b, a % b); }
 
 template <int D_, int NT_, int KV_, int IO_>
 struct Traits {
     static constexpr int D = D_, NT = NT_, KV = KV_, IO = IO_;
     // FP8 pages with one query-head tile: more consumer warps (the E4M3
     // expansion makes the consumers, not the copies, set the pace)
-    static constexpr bool FP4 = KV_ == kFP4;
-    // pages read as codes straight into registers, whose fragments leave O^T and
-    // the merge rows in the order of fp8_out_d / fp4_out_d
-    static constexpr bool CODES = KV_ == kFP8 || FP4;
-    static constexpr int W = FP4 ? VW_DECODE_FP4_WARPS
-                                 : (KV_ == kFP8 && NT_ == 1) ? kFp8ConsumerWarps : kConsumerWarps;
-    static constexpr int PW = FP4 ? VW_DECODE_FP4_PRODUCERS
-                                  : KV_ == kFP8 ? kFp8ProducerWarps : 1;   // producer warps W..W+PW-1
-    static constexpr int IPW = FP4 ? VW_DECODE_FP4_ISSUERS
-                                   : KV_ == kFP8 ? kFp8Issuers : kIssuers;  // issuing lanes per producer warp
+    static constexpr int W = (KV_ == kFP8 && NT_ == 1) ? kFp8ConsumerWarps : kConsumerWarps;
+    static constexpr int PW = KV_ == kFP8 ? kFp8ProducerWarps : 1;   // producer warps W..W+PW-1
+    static constexpr int IPW = KV_ == kFP8 ? kFp8Issuers : kIssuers;  // issuing lanes per producer warp
     static constexpr int NI = PW * IPW;                               // issuers in all
     static constexpr int THREADS = (W + PW) * 32;
     static constexpr int G = 8 * NT;                         // padded query heads per KV head
     static constexpr int EB = KV == kFP8 ? 1 : 2;            // pool element bytes
     static constexpr int ROW = D * EB;                       // bytes of one token row
     static constexpr int CHUNKS = ROW / 128;                 // 128-B swizzle columns per row
-    // one page-head: K rows 0-15, V 16-31 (4-bit pages: one record)
-    static constexpr int STAGE = FP4 ? Fp4Rec<D>::BYTES : 32 * ROW;
+    static constexpr int STAGE = 32 * ROW;                   // one page-head: K rows 0-15, V 16-31
     static constexpr int SCAL = KV == kFP8 ? 128 : 0;        // K and V scales of a page-head
-    static constexpr bool MMA_BF16 = KV == kBF16;            // FP8 and 4-bit pages compute in f16
+    static constexpr bool MMA_BF16 = KV == kBF16;            // FP8 pages compute in f16
     // P as a pair hi + lo of the MMA type, two P V MMAs: a single bf16 (2^-9)
     // or f16 x V-scale (2^-11) probability puts outputs whose few large V terms
     // cancel outside max-abs 2e-3 / rel 1e-2; f16 pools keep a single f16 P
-    static constexpr bool PSPLIT = KV == kBF16 || CODES;
+    static constexpr bool PSPLIT = KV == kBF16 || KV == kFP8;
     // FP8 pages: the V codes are read after the softmax (not with the K codes)
     // when registers are short -- two query-head tiles, or more than four
     // consumer warps -- so that the K and V codes are never live together
@@ -185,7 +168,7 @@ struct Traits {
     // (lanes 4g+c hold query heads 2c, 2c+1, d values 32 apart) then fall on 32
     // different banks.  2-byte pages keep rows of D (a 4-way conflict measured
     // cheaper than the padded rows).
-    static constexpr int MROW = CODES ? D + 4 : D;
+    static constexpr int MROW = KV == kFP8 ? D + 4 : D;
     // the warp states are merged one 8-head tile at a time: [W][8] rows of
     // MROW + 2 floats (o, max, sum), then [W + 2][8] weights, max and sum
     static constexpr int MERGE = W * 8 * (MROW + 2) * 4 + (W + 2) * 8 * 4;
@@ -200,7 +183,7 @@ struct Traits {
                                  align_up_c(QS * QSLOT, 1024) + PFX + PW * 1024 + 1024;
     // resident CTAs per SM the shared memory is sized for: FP8 pages and two
     // query-head tiles need the larger stages and registers of two
-    static constexpr int RES = (NT == 1 && !CODES) ? kCtasPerSm : 2;
+    static constexpr int RES = (NT == 1 && KV != kFP8) ? kCtasPerSm : 2;
     static constexpr int SMEM_CAP = smem_per_cta(RES);
     static constexpr int BUDGET = SMEM_CAP - 1024 /* base alignment slack */ -
                                   (SCAL ? 1024 : 0) /* scale ring alignment */;
@@ -223,14 +206,13 @@ struct Traits {
     // registers (the bound of 3 CTAs' worth of threads), which leaves every SM
     // sub-partition room for the single-warp combine CTAs that wait beside the
     // decode CTAs; the others keep 168 (2 CTAs' worth) to avoid spills.
-    static constexpr int MIN_CTAS = (NT == 1 && !CODES) ? VW_DECODE_MIN_CTAS_2B : 2;
+    static constexpr int MIN_CTAS = (NT == 1 && KV != kFP8) ? VW_DECODE_MIN_CTAS_2B : 2;
     static_assert(CHUNKS >= 1, "row must be at least 128 bytes");
     static_assert(S >= 4, "too few pipeline stages");
     static_assert(S % W == 0 && S % NI == 0, "stage ownership needs S % W == S % issuers == 0");
     static_assert(32 % NI == 0 && IPW <= 32, "issuers must divide the 32-page batch");
     static_assert(SMEM <= SMEM_CAP, "shared memory over the per-CTA limit");
-    static_assert(FP4 || STAGE % 1024 == 0, "1024-B tile alignment");
-    static_assert(STAGE % 16 == 0, "bulk copies of whole 16-B units");
+    static_assert(STAGE % 1024 == 0, "1024-B tile alignment");
 };
 
 // Page as the producer publishes it to its issuing lanes: TMA row of its first
@@ -296,105 +278,6 @@ __device__ __forceinline__ uint32_t swz16(int row, int d) {
 // Same for 1-byte rows of 128 (FP8, D = 128): [32 rows][128 B].
 __device__ __forceinline__ uint32_t swz8(int row, int d) {
     return (uint32_t)(row * 128 + ((((d & 127) >> 4) ^ (row & 7)) << 4) + (d & 15));
-}
-
-// Largest b with Hkv * pfx[b] <= x (x < Hkv * pfx[B]).
-__device__ __forceinline__ int find_seq(const int* pfx, int B, int Hkv, long long x) {
-    int lo = 0, hi = B - 1;
-    while (lo < hi) {
-        int mid = (lo + hi + 1) >> 1;
-        if ((long long)Hkv * pfx[mid] <= x) lo = mid; else hi = mid - 1;
-    }
-    return lo;
-}
-
-// Page ranges of the decode CTAs.  The (sequence b, KV head h) segments,
-// ordered by (b, h), lie end to end.  A CTA that crosses a segment boundary
-// pays for a second query tile, a merge of its warps' states and a partial
-// write, and it is the one that finishes last; so each segment is followed by
-// a gap of `cost` virtual pages (DecodeParams::seg_cost) and the virtual line
-// is cut into equal lengths vper.  Page x of the segment with ordinal k (among
-// segments with pages) sits at v(x) = x + cost * k; CTA c takes the pages
-// whose v falls in [c * vper, (c + 1) * vper), so the CTA holding page x is
-// v(x) / vper.  With cost 0 this is the plain equal split.  The decode, its
-// combine grid and the plan all cut with the launch's cost.
-
-// Virtual positions stay far below 2^31: a launch covers fewer than 2^26 pages
-// (the pool's rows are checked against 2^31 at creation) plus at most
-// kMaxSegmentCost per segment.
-__host__ __device__ __forceinline__ int virtual_total(int total_pages, int segments, int cost) {
-    return total_pages + cost * segments;
-}
-__host__ __device__ __forceinline__ int virtual_per_cta(int vtotal, int grid) {
-    const int v = (vtotal + grid - 1) / grid;
-    return v < kMinPagesPerCta ? kMinPagesPerCta : v;
-}
-
-// First page x with v(x) >= t (total when there is none), from the exclusive
-// prefixes of pages (pfx) and of sequences with pages (nzp) over B sequences.
-__device__ __forceinline__ int range_start(const int* pfx, const int* nzp, int B, int Hkv, int cost, int t) {
-    const int total = Hkv * pfx[B];
-    if (t >= virtual_total(total, Hkv * nzp[B], cost)) return total;
-    // largest b whose first virtual position is <= t (always a sequence with pages)
-    int lo = 0, hi = B - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (virtual_total(Hkv * pfx[mid], Hkv * nzp[mid], cost) <= t) lo = mid; else hi = mid - 1;
-    }
-    const int np = pfx[lo + 1] - pfx[lo];
-    const int r = t - virtual_total(Hkv * pfx[lo], Hkv * nzp[lo], cost);
-    const int h = r / (np + cost);
-    const int off = r - h * (np + cost);
-    // inside the gap after segment h: the range starts at the next segment
-    return Hkv * pfx[lo] + h * np + (off < np ? off : np);
-}
-
-__device__ __forceinline__ void set_err(uint32_t* err, uint32_t bit) { atomicOr(err, bit); }
-
-// Pages per sequence -> exclusive prefixes of pages (pfx) and of sequences with
-// pages (nzp), by one warp, 32 sequences at a time, keeping each seq_len in
-// slen when given.  A seq_len of 0 gives no pages and one longer than its
-// block-table row is clamped to the row; both are flagged when `report`.  With
-// WIN only the pages that the window and the sinks leave visible count.
-template <bool WIN>
-__device__ __forceinline__ void warp_prefixes(const uint32_t* seq_lens, int B, int bt_stride,
-                                              uint32_t* err, bool report, int* pfx, int* nzp,
-                                              int* slen, int lane, uint32_t window, uint32_t sinks) {
-    int run = 0, run_nz = 0;
-    if (lane == 0) { pfx[0] = 0; nzp[0] = 0; }
-    for (int base_b = 0; base_b < B; base_b += 32) {
-        const int b = base_b + lane;
-        int np = 0;
-        if (b < B) {
-            const int sl = (int)__ldg(seq_lens + b);
-            if (slen) slen[b] = sl;
-            np = (sl + 15) >> 4;
-            if (sl <= 0 || np > bt_stride) {
-                if (report) set_err(err, kDevErrSeqLen);
-                np = sl <= 0 ? 0 : bt_stride;
-            }
-            if (WIN && np > 0) np = decode_span(sl, bt_stride, window, sinks).n;
-        }
-        int incl = np, incl_nz = np > 0 ? 1 : 0;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, off);
-            const int vz = __shfl_up_sync(0xffffffffu, incl_nz, off);
-            if (lane >= off) { incl += v; incl_nz += vz; }
-        }
-        if (b < B) { pfx[b + 1] = run + incl; nzp[b + 1] = run_nz + incl_nz; }
-        run += __shfl_sync(0xffffffffu, incl, 31);
-        run_nz += __shfl_sync(0xffffffffu, incl_nz, 31);
-    }
-}
-
-template <int IO>
-__device__ __forceinline__ float io_to_f32(uint32_t h) {
-    return IO == kBF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
-}
-template <int IO>
-__device__ __forceinline__ uint16_t f32_to_io(float f) {
-    return IO == kBF16 ? f32_to_bf16_bits(f) : f32_to_f16_bits(f);
 }
 
 // ------------------------------------------------------------------ producer
@@ -473,19 +356,6 @@ __device__ void producer(const CUtensorMap* tmap, const DecodeParams& p, const S
         if (ii == 0) VW_TRACE(2, globaltimer());
         if (ii == n - 1) VW_TRACE(4, globaltimer());
         uint8_t* st = sm.stages + s * T::STAGE;
-        if constexpr (T::FP4) {
-            if (pi.row0 >= 0) {
-                mbar_arrive_expect_tx(&sm.full[s], T::STAGE);
-                bulk_load(st, p.kv_data + (size_t)(pi.row0 >> 5) * T::STAGE, T::STAGE, &sm.full[s]);
-            } else {
-                // invalid block id: a record of zeros (as FP8 scales below)
-                for (int k = 0; k < T::STAGE / 16; ++k) reinterpret_cast<uint4*>(st)[k] = make_uint4(0, 0, 0, 0);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&sm.full[s]);
-            }
-            issued_hi = ii;
-            return true;
-        }
         if constexpr (T::KV == kFP8) {
             float* sc = sm.scal + s * 32;
             if (pi.row0 >= 0) {
@@ -618,52 +488,6 @@ __device__ void producer(const CUtensorMap* tmap, const DecodeParams& p, const S
     }
 }
 
-// Merge of the split-K pieces of one segment (b, h) for query head j and
-// output elements d..d+3: the pieces (o, max, sum) left by decode CTAs
-// c0..c0+n-1 (CTA c0 in slot slot0, the others in slot 0) are weighted by
-// 2^(max_c - max), the online-softmax rule of flash_attention.bm:149-157
-// applied across pieces; up to kCombineBatch pieces per memory round trip.
-constexpr int kCombineBatch = 8;
-
-template <int D, int G, int IO>
-__device__ __forceinline__ void merge_unit(const DecodeParams& p, int b, int h, int j, int d, int c0,
-                                           int n, int slot0, float vfold) {
-    uint16_t* out = reinterpret_cast<uint16_t*>(p.out);
-    const int g = (int)p.group;
-    float M = -INFINITY, Ls = 0.0f, a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
-    for (int k0 = 0; k0 < n; k0 += kCombineBatch) {
-        float2 ml[kCombineBatch];
-        float4 o[kCombineBatch];
-#pragma unroll
-        for (int k = 0; k < kCombineBatch; ++k) {
-            ml[k] = make_float2(-INFINITY, 0.0f);
-            o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (k0 + k < n) {
-                const int c = c0 + k0 + k;
-                const size_t piece = (size_t)c * 2 + (c == c0 ? slot0 : 0);
-                ml[k] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (piece * G + j) * 2));
-                o[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (piece * G + j) * D + d));
-            }
-        }
-        float Mn = M;
-#pragma unroll
-        for (int k = 0; k < kCombineBatch; ++k) Mn = fmaxf(Mn, ml[k].x);
-        const float r = M > -INFINITY ? ex2(M - Mn) : 0.0f;
-        Ls *= r; a0 *= r; a1 *= r; a2 *= r; a3 *= r;
-#pragma unroll
-        for (int k = 0; k < kCombineBatch; ++k) {
-            const float w = ml[k].x > -INFINITY ? ex2(ml[k].x - Mn) : 0.0f;
-            Ls += ml[k].y * w;
-            a0 += o[k].x * w; a1 += o[k].y * w; a2 += o[k].z * w; a3 += o[k].w * w;
-        }
-        M = Mn;
-    }
-    const float r = vfold / Ls;
-    const uint32_t lo = (uint32_t)f32_to_io<IO>(a0 * r) | ((uint32_t)f32_to_io<IO>(a1 * r) << 16);
-    const uint32_t hi = (uint32_t)f32_to_io<IO>(a2 * r) | ((uint32_t)f32_to_io<IO>(a3 * r) << 16);
-    *reinterpret_cast<uint2*>(out + ((size_t)b * p.Hq + (size_t)h * g + j) * D + d) = make_uint2(lo, hi);
-}
-
 // ------------------------------------------------------------------ consumer
 
 // Query fragments (B operand of S^T = K Q^T) from the staged query tile.
@@ -682,26 +506,24 @@ __device__ __forceinline__ void load_q(const DecodeParams& p, const uint8_t* qti
         const int j = nt * 8 + (lane >> 2);
         const bool live = j < (int)p.group;
         const uint8_t* row = qtile + (live ? j : 0) * T::D * 2;
-        if constexpr (T::CODES) {
-            // lane c holds elements c*D/4 .. +D/4-1
+        if constexpr (T::KV == kFP8) {
             const int c = lane & 3;
-            constexpr int NW = T::D / 8;
-            uint32_t w[NW];
+            uint32_t w[16];
 #pragma unroll
-            for (int u = 0; u < NW / 4; ++u) {
-                const uint4 v = live ? *reinterpret_cast<const uint4*>(row + c * (T::D / 2) + u * 16)
+            for (int u = 0; u < 4; ++u) {
+                const uint4 v = live ? *reinterpret_cast<const uint4*>(row + c * 64 + u * 16)
                                      : make_uint4(0, 0, 0, 0);
                 w[4 * u] = v.x; w[4 * u + 1] = v.y; w[4 * u + 2] = v.z; w[4 * u + 3] = v.w;
             }
             if (p.rope_theta > 0.0f) {
                 const bool lo = c < 2;                  // elements below D/2
 #pragma unroll
-                for (int m = 0; m < NW; ++m) {
+                for (int m = 0; m < 16; ++m) {
                     const uint32_t other = __shfl_xor_sync(0xffffffffu, w[m], 2);
                     const uint32_t rw = lo ? w[m] : other, iw = lo ? other : w[m];
                     float r0 = io_to_f32<T::IO>(rw & 0xFFFFu), i0 = io_to_f32<T::IO>(iw & 0xFFFFu);
                     float r1 = io_to_f32<T::IO>(rw >> 16), i1 = io_to_f32<T::IO>(iw >> 16);
-                    const int d = (c & 1) * (T::D / 4) + 2 * m;   // index of the lower element
+                    const int d = (c & 1) * 32 + 2 * m;   // index of the lower element
                     rope_pair(r0, i0, d, T::D, p.rope_theta, pos);
                     rope_pair(r1, i1, d + 1, T::D, p.rope_theta, pos);
                     w[m] = lo ? ((uint32_t)f32_to_io<T::IO>(r0) | ((uint32_t)f32_to_io<T::IO>(r1) << 16))
@@ -709,16 +531,15 @@ __device__ __forceinline__ void load_q(const DecodeParams& p, const uint8_t* qti
                 }
             }
 #pragma unroll
-            for (int m = 0; m < NW; ++m) {
+            for (int m = 0; m < 16; ++m) {
                 if constexpr (T::IO == kBF16)       // pages compute in f16
                     w[m] = pack2<false>(bf16_bits_to_f32(w[m] & 0xFFFFu), bf16_bits_to_f32(w[m] >> 16));
             }
             // k-step kt: elements 32c+4kt+1, +3 first, then +0, +2 (the K pairs)
 #pragma unroll
             for (int kt = 0; kt < T::KT; ++kt) {
-                // (4-bit pages: the pairs in their own order)
-                qf[nt][kt][0] = T::FP4 ? w[2 * kt] : __byte_perm(w[2 * kt], w[2 * kt + 1], 0x7632u);
-                qf[nt][kt][1] = T::FP4 ? w[2 * kt + 1] : __byte_perm(w[2 * kt], w[2 * kt + 1], 0x5410u);
+                qf[nt][kt][0] = __byte_perm(w[2 * kt], w[2 * kt + 1], 0x7632u);
+                qf[nt][kt][1] = __byte_perm(w[2 * kt], w[2 * kt + 1], 0x5410u);
             }
         } else {
 #pragma unroll
@@ -764,16 +585,7 @@ __device__ __forceinline__ void append_row(const DecodeParams& p, uint8_t* stage
         // pool row of (layer, block, head, kv, t) in [L][NB][Hkv][2][16]
         const size_t prow = ((((size_t)p.layer * p.num_blocks + blk) * p.Hkv + h) * 2 + kv) * 16 + t;
         const int srow = kv * 16 + t;
-        if constexpr (T::FP4) {
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int k = 0; k < PER / 2; ++k) {
-                v[2 * k] = io_to_f32<T::IO>(nkv[kv][k] & 0xFFFFu);
-                v[2 * k + 1] = io_to_f32<T::IO>(nkv[kv][k] >> 16);
-            }
-            uint8_t* rec = p.kv_data + (((size_t)p.layer * p.num_blocks + blk) * p.Hkv + h) * T::STAGE;
-            fp4_store_row<T::D>(stage, blk_ok ? rec : nullptr, kv, t, lane, v);
-        } else if constexpr (T::KV != kFP8) {
+        if constexpr (T::KV != kFP8) {
             const uint32_t* w = nkv[kv];
             uint8_t* gdst = p.kv_data + prow * T::ROW + lane * PER * 2;
             uint8_t* sdst = stage + swz16(srow, lane * PER);
@@ -810,15 +622,6 @@ __device__ __forceinline__ void append_row(const DecodeParams& p, uint8_t* stage
 // NaN/Inf through 0 * garbage in the P.V product.
 template <class T>
 __device__ __forceinline__ void zero_rows(uint8_t* stage, int from, int to, int lane) {
-    if constexpr (T::FP4) {
-        using R = Fp4Rec<T::D>;
-        // (codes and scales: a code of 0 times a NaN scale is NaN)
-        for (int k = lane; k < (to - from) * (R::CODE_ROW / 16); k += 32)
-            reinterpret_cast<uint4*>(stage + R::V + from * R::CODE_ROW)[k] = make_uint4(0, 0, 0, 0);
-        for (int k = lane; k < (to - from) * R::GROUPS; k += 32)
-            stage[R::VS + k % R::GROUPS * 16 + from + k / R::GROUPS] = 0;
-        return;
-    }
     const int per_row = T::CHUNKS * 8;                   // 16-B pieces per row
     const int total = (to - from) * per_row;
     for (int k = lane; k < total; k += 32) {
@@ -868,72 +671,6 @@ __device__ __forceinline__ void load_fp8_codes(const uint8_t* st, int lane, int 
     }
 }
 
-// 4-bit page-head fragments (D elements; the record in vw_fp4.cuh).  The A rows of
-// S^T = K Q^T and the columns of V^T are tokens in an order of our choosing,
-// fp4_token(r) = r ^ (r/2 & 1): two rows that lanes of one load phase read then lie an odd
-// number of rows apart, which halves the bank conflicts of the V loads.
-//  * K: lane (g, c) takes the D/4 codes c*D/4 .. of token rows g and g+8; k-step kt uses its
-//    codes 4kt .. 4kt+3 (the reduction order inside a k-step is free), so its
-//    scales are those of one or two groups only.
-//  * V: lane (g, c) takes the D/8 codes g*D/8 .. of token rows 2c, 2c+1, 2c+8, 2c+9; the
-//    codes of two rows interleave into bytes that convert to a pair (two tokens,
-//    one element) at once; row r of d-tile mt is fp4_out_d(r, mt).
-__device__ __forceinline__ int fp4_token(int r) { return r ^ ((r >> 1) & 1); }
-
-template <int D>
-__host__ __device__ __forceinline__ int fp4_out_d(int r, int mt) {
-    return (D / 8) * (r & 7) + (D / 16) * (r >> 3) + mt;
-}
-
-template <int D>
-struct Fp4Codes {
-    uint32_t k[2][D / 32];     // codes of token rows g, g+8
-    uint32_t v[4][D / 64];     // of token rows 2c, 2c+1, 2c+8, 2c+9
-    uint32_t ks[2][D / 64];    // K scales, each twice (f16 pair), of the lane's one or two groups
-    uint32_t vs[2];            // V scales of the token pairs (f16 pairs)
-};
-
-template <int D>
-__device__ __forceinline__ void load_fp4_codes(const uint8_t* st, int lane, Fp4Codes<D>& f) {
-    using R = Fp4Rec<D>;
-    const int g = lane >> 2, c = lane & 3;
-#pragma unroll
-    for (int rr = 0; rr < 2; ++rr) {
-        const int tok = fp4_token(g) + 8 * rr;
-        const uint8_t* kp = st + tok * R::CODE_ROW + c * (D / 8);
-        if constexpr (D == 128) {
-            const uint4 w = *reinterpret_cast<const uint4*>(kp);
-            f.k[rr][0] = w.x; f.k[rr][1] = w.y; f.k[rr][2] = w.z; f.k[rr][3] = w.w;
-            const uint32_t s = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(st + R::KS + tok * R::GROUPS + 2 * c));
-            f.ks[rr][0] = __byte_perm(s, s, 0x1010u);
-            f.ks[rr][1] = __byte_perm(s, s, 0x3232u);
-        } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(kp);
-            f.k[rr][0] = w.x; f.k[rr][1] = w.y;
-            const uint32_t s = e4m3x2_to_f16x2(st[R::KS + tok * R::GROUPS + c]);
-            f.ks[rr][0] = __byte_perm(s, s, 0x1010u);
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int tok = fp4_token(2 * c + (r & 1)) + 8 * (r >> 1);
-        const uint8_t* vp = st + R::V + tok * R::CODE_ROW + g * (D / 16);
-        if constexpr (D == 128) {
-            const uint2 w = *reinterpret_cast<const uint2*>(vp);
-            f.v[r][0] = w.x; f.v[r][1] = w.y;
-        } else {
-            f.v[r][0] = *reinterpret_cast<const uint32_t*>(vp);
-        }
-    }
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        // tokens 2c, 2c+1 of the group, in the order of the rows above
-        const uint32_t s = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(
-            st + R::VS + (D == 128 ? g : g >> 1) * 16 + 8 * q + 2 * c));
-        f.vs[q] = __byte_perm(s, s, (c & 1) ? 0x1032u : 0x3210u);
-    }
-}
-
 __device__ __forceinline__ uint32_t word_of(const uint4& h, int k) {
     return k == 0 ? h.x : k == 1 ? h.y : k == 2 ? h.z : h.w;
 }
@@ -949,11 +686,10 @@ __host__ __device__ __forceinline__ int fp8_out_d(int r, int mt) {
 // 16 apart in one store (lanes g = 0..7); flipping bits 0-2 of d by bits 4-6
 // spreads them over the banks, and with the rows of D + 4 floats of the four
 // query-head pairs a store's 32 lanes meet 32 different banks (a permutation
-// inside each block of 16).  head_dim 64 (4-bit pages): d values 8 apart, bits
-// 0-2 flipped by bits 3-5.
+// inside each block of 16).
 template <class T>
 __device__ __forceinline__ int merge_col(int d) {
-    return T::CODES ? d ^ ((d / (T::D / 8)) & 7) : d;
+    return T::KV == kFP8 ? d ^ ((d >> 4) & 7) : d;
 }
 
 template <class T, bool WIN>
@@ -971,7 +707,7 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
     const int mi = lane >> 3;
     const int k_tok = (lane & 7) + ((mi & 1) << 3), k_hs = mi >> 1;
     const int v_tok = (lane & 7) + ((mi >> 1) << 3), v_hs = mi & 1;
-    const int t0 = T::FP4 ? fp4_token(lane >> 2) : lane >> 2, t1 = t0 + 8;
+    const int t0 = lane >> 2, t1 = t0 + 8;
 
     bool alive = true;
     int seg_k = 0;
@@ -1097,12 +833,6 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
             float ks0 = 1.0f, ks1 = 1.0f, vs0 = 1.0f, vs1 = 1.0f;
             const uint32_t tbase = smem_u32(st);
             Fp8Codes fc;
-            Fp4Codes<T::D> f4;
-            if constexpr (T::FP4) {
-                load_fp4_codes<T::D>(st, lane, f4);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.empty[s]);
-            }
             if constexpr (T::KV == kFP8) {
                 // this lane's codes and scales are all the page-head it needs:
                 // the stage goes back to the producer before any math, or, with
@@ -1126,14 +856,7 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
 #pragma unroll
             for (int kt = 0; kt < T::KT; ++kt) {
                 uint32_t a0, a1, a2, a3;
-                if constexpr (T::FP4) {
-                    uint32_t r0[4], r1[4];
-                    fp4x8_to_f16(f4.k[0][kt >> 1], r0);
-                    fp4x8_to_f16(f4.k[1][kt >> 1], r1);
-                    const int j = 2 * (kt & 1), gi = T::D == 128 ? kt >> 2 : 0;
-                    a0 = f16x2_mul(r0[j], f4.ks[0][gi]); a1 = f16x2_mul(r1[j], f4.ks[1][gi]);
-                    a2 = f16x2_mul(r0[j + 1], f4.ks[0][gi]); a3 = f16x2_mul(r1[j + 1], f4.ks[1][gi]);
-                } else if constexpr (T::KV == kFP8) {
+                if constexpr (T::KV == kFP8) {
                     const uint32_t w0 = run_word(fc.k[0], kt), w1 = run_word(fc.k[1], kt);
                     a0 = fp8_pair_odd(w0); a1 = fp8_pair_odd(w1);
                     a2 = fp8_pair_even(w0); a3 = fp8_pair_even(w1);
@@ -1224,30 +947,10 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.empty[s]);
             }
-            uint32_t ve[2][2][T::FP4 ? T::D / 64 : 1];     // interleaved V codes [even, odd][token pair][word]
-            if constexpr (T::FP4) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int k = 0; k < T::D / 64; ++k)
-                        fp4_interleave(f4.v[2 * q][k], f4.v[2 * q + 1][k], ve[0][q][k], ve[1][q][k]);
-            }
 #pragma unroll
             for (int mt = 0; mt < T::MT; ++mt) {
                 uint32_t a0, a1, a2, a3;
-                if constexpr (T::FP4) {
-                    // elements mt and MT + mt of the lane's run
-                    uint32_t r[4];
-                    const int x1 = T::MT + mt;
-                    fp4x8_to_f16(ve[mt & 1][0][0], r);
-                    a0 = f16x2_mul(r[mt >> 1 & 3], f4.vs[0]);
-                    fp4x8_to_f16(ve[x1 & 1][0][x1 >> 3], r);
-                    a1 = f16x2_mul(r[(x1 & 7) >> 1], f4.vs[0]);
-                    fp4x8_to_f16(ve[mt & 1][1][0], r);
-                    a2 = f16x2_mul(r[mt >> 1 & 3], f4.vs[1]);
-                    fp4x8_to_f16(ve[x1 & 1][1][x1 >> 3], r);
-                    a3 = f16x2_mul(r[(x1 & 7) >> 1], f4.vs[1]);
-                } else if constexpr (T::KV == kFP8) {
+                if constexpr (T::KV == kFP8) {
                     // byte mt of unit g: d = 16g + mt (rows g) and 16g + 8 + mt (rows g + 8)
                     const int lo = mt >> 2, hi = 2 + (mt >> 2), j = mt & 3;
                     a0 = fp8_pair_cross(word_of(fc.v[0], lo), word_of(fc.v[1], lo), j);
@@ -1266,7 +969,7 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
                 }
             }
             __syncwarp();
-            if constexpr (!T::CODES) {
+            if constexpr (T::KV != kFP8) {
                 if (lane == 0) mbar_arrive(&sm.empty[s]);
             }
         }
@@ -1295,9 +998,8 @@ __device__ void consumer(const DecodeParams& p, const Smem& sm, int begin, int e
 #pragma unroll
             for (int mt = 0; mt < T::MT; ++mt) {
                 // O^T rows lane/4 and lane/4 + 8 of d-tile mt
-                const int r0 = lane >> 2;
-                const int dA = T::FP4 ? fp4_out_d<T::D>(r0, mt) : T::KV == kFP8 ? fp8_out_d(r0, mt) : mt * 16 + r0;
-                const int dB = T::FP4 ? fp4_out_d<T::D>(r0 + 8, mt) : T::KV == kFP8 ? fp8_out_d(r0 + 8, mt) : dA + 8;
+                const int dA = T::KV == kFP8 ? fp8_out_d(lane >> 2, mt) : mt * 16 + (lane >> 2);
+                const int dB = T::KV == kFP8 ? fp8_out_d((lane >> 2) + 8, mt) : dA + 8;
                 mo[jl * T::MROW + merge_col<T>(dA)] = o[nt][mt][0];
                 mo[(jl + 1) * T::MROW + merge_col<T>(dA)] = o[nt][mt][1];
                 mo[jl * T::MROW + merge_col<T>(dB)] = o[nt][mt][2];
@@ -1407,7 +1109,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p) {
         }
         if (warp >= T::W) {
             // every producer warp takes the first batch into its own buffer
-            if (!T::FP4 && lane == 0) prefetch_tensormap(&tmap);
+            if (lane == 0) prefetch_tensormap(&tmap);
             if (warp == T::W && lane < 3) sm.flag[2 + lane] = __ldcg(entry + lane);
             const int4 rec = __ldcg(reinterpret_cast<const int4*>(entry + 4) + lane);
             PageInfo pi;
@@ -1418,7 +1120,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p) {
             sm.pinfo[(warp - T::W) * 64 + lane] = pi;
         }
     } else if (warp == T::W) {
-        if (!T::FP4 && lane == 0) prefetch_tensormap(&tmap);
+        if (lane == 0) prefetch_tensormap(&tmap);
         warp_prefixes<WIN>(p.seq_lens, (int)p.B, (int)p.bt_stride, p.err, blockIdx.x == 0, sm.pfx, sm.nzp,
                            sm.slen, lane, p.window, p.sinks);
     }
@@ -1461,90 +1163,6 @@ decode_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p) {
         consumer<T, WIN>(p, sm, begin, end, deadline);
     }
     if (threadIdx.x == 0) VW_TRACE(7, globaltimer());
-}
-
-// ------------------------------------------------------------------ combine
-
-// The combine grid is resident next to the decode grids of this layer and the
-// next one (it launches before the decode grid ends and waits in
-// griddepcontrol.wait), so its CTAs must fit beside two decode CTAs.  The
-// register file is split over the SM's four sub-partitions (16,384 each); ten
-// 128-register decode warps leave 4,096 in a sub-partition holding three of
-// them, so a combine CTA is a single warp of at most 80 registers (2,560),
-// and it runs with the decode's shared-memory carveout.  CTA (segment, j) merges query head j of the
-// segment, four output elements per lane.
-constexpr int kCombineWarps = 1;
-constexpr int kCombineThreads = kCombineWarps * 32;
-constexpr int kCombineMinBlocks = 25;  // 65,536 / (32 x 25) -> a cap of 80 registers
-
-// Merge of the split-K partials, one CTA per (sequence, KV head) segment.  The
-// CTA recomputes the decode grid's page ranges from seq_lens (same clamping,
-// same per-CTA quantum), returns at once for a segment that one decode CTA
-// finished, and otherwise merges the pieces (o, max, sum) left by decode CTAs
-// c0..c1 with weights 2^(max_c - max) -- the merge rule of the online softmax
-// in flash_attention.bm:149-157, applied across pieces instead of tokens.
-// Launched as a programmatic dependent of its decode grid: the geometry is
-// computed while the decode still runs, the partials are read after
-// griddepcontrol.wait.  Each thread produces four consecutive output elements.
-template <int D, int G, int IO, bool WIN>
-__global__ void __launch_bounds__(kCombineThreads, kCombineMinBlocks) combine_kernel(const DecodeParams p, int dec_grid,
-                                                                  float vfold) {
-    __shared__ int red[kCombineThreads / 32][4];
-    if (threadIdx.x == 0) VW_TRACE(12, globaltimer());
-    // the next grid (the following layer's decode) may start its prologue now;
-    // it waits for this whole grid before it writes anything this grid reads
-    griddep_launch_dependents();
-    const int Hkv = (int)p.Hkv;
-    const int b = (int)blockIdx.x / Hkv, h = (int)blockIdx.x - b * Hkv;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    auto pages = [&](int i) {
-        const int sl = (int)__ldcg(p.seq_lens + i);
-        const int np = (sl + 15) >> 4;
-        if (WIN && sl > 0) return decode_span(sl, (int)p.bt_stride, p.window, p.sinks).n;
-        return sl <= 0 ? 0 : min(np, (int)p.bt_stride);
-    };
-    // pages and sequences with pages, before b and in all (the decode's prefixes)
-    int before = 0, all = 0, nz_before = 0, nz_all = 0;
-    for (int i = threadIdx.x; i < (int)p.B; i += kCombineThreads) {
-        const int np = pages(i);
-        all += np;
-        nz_all += np > 0;
-        if (i < b) { before += np; nz_before += np > 0; }
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        before += __shfl_xor_sync(0xffffffffu, before, off);
-        all += __shfl_xor_sync(0xffffffffu, all, off);
-        nz_before += __shfl_xor_sync(0xffffffffu, nz_before, off);
-        nz_all += __shfl_xor_sync(0xffffffffu, nz_all, off);
-    }
-    if (lane == 0) { red[warp][0] = before; red[warp][1] = all; red[warp][2] = nz_before; red[warp][3] = nz_all; }
-    __syncthreads();
-    before = all = nz_before = nz_all = 0;
-#pragma unroll
-    for (int w = 0; w < kCombineThreads / 32; ++w) {
-        before += red[w][0]; all += red[w][1]; nz_before += red[w][2]; nz_all += red[w][3];
-    }
-    const int np = pages(b);
-    if (np == 0) return;
-    const int cost = (int)p.seg_cost;
-    const int vper = virtual_per_cta(virtual_total(Hkv * all, Hkv * nz_all, cost), dec_grid);
-    const int s_begin = Hkv * before + h * np;
-    const int k = Hkv * nz_before + h;        // segment ordinal
-    const int v0 = s_begin + cost * k;
-    const int c0 = v0 / vper, c1 = (v0 + np - 1) / vper;
-    if (c0 == c1) return;                      // written out by the decode CTA itself
-    // CTA c0 holds this segment in slot 0 when the segment starts its range
-    // (the page before it, of segment k-1, lies in an earlier CTA), else in
-    // slot 1 (its last segment); every later CTA starts inside it
-    const int slot0 = (k == 0 || (s_begin - 1) + cost * (k - 1) < c0 * vper) ? 0 : 1;
-    griddep_wait();
-    if (threadIdx.x == 0) VW_TRACE(13, globaltimer());
-    const int g = (int)p.group;
-    const int n = c1 - c0 + 1;
-    const int j = (int)blockIdx.y * kCombineWarps + warp, d = lane * 4;
-    if (j < g && d < D) merge_unit<D, G, IO>(p, b, h, j, d, c0, n, slot0, vfold);
-    if (threadIdx.x == 0) VW_TRACE(14, globaltimer());
 }
 
 
@@ -1610,20 +1228,6 @@ cudaError_t launch_decode_plan(const DecodeParams& p, int grid, int* plan, cudaS
 namespace {
 
 template <class T, bool WIN>
-cudaError_t launch_combine(const DecodeLaunch& L) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(L.p.B * L.p.Hkv, (L.p.group + kCombineWarps - 1) / kCombineWarps);
-    cfg.blockDim = dim3(kCombineThreads);
-    cfg.stream = L.stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, combine_kernel<T::D, T::G, T::IO, WIN>, L.p, L.grid, T::VFOLD);
-}
-
-template <class T, bool WIN>
 cudaError_t launch_t(const DecodeLaunch& L) {
     // the dynamic-smem opt-in is per device; remember it per device ordinal
     static std::atomic<uint64_t> configured{0};
@@ -1657,7 +1261,7 @@ cudaError_t launch_t(const DecodeLaunch& L) {
     }
     cudaError_t e = cudaLaunchKernelEx(&cfg, decode_kernel<T, WIN>, *L.tmap, L.p);
     if (e != cudaSuccess) return e;
-    return launch_combine<T, WIN>(L);
+    return launch_combine<T::D, T::G, T::IO, WIN>(L, T::VFOLD);
 }
 
 template <int D, int KV, int IO>
@@ -1693,10 +1297,7 @@ extern "C" __attribute__((visibility("default"))) int vw_debug_trace(void* host,
 
 cudaError_t launch_paged_decode(const DecodeLaunch& L) {
     const uint32_t D = L.head_dim;
-    if (L.kv_kind == kFP4) {
-        if (D == 64) return L.io_kind == kBF16 ? launch_d<64, kFP4, kBF16>(L) : launch_d<64, kFP4, kF16>(L);
-        return L.io_kind == kBF16 ? launch_d<128, kFP4, kBF16>(L) : launch_d<128, kFP4, kF16>(L);
-    }
+    if (L.kv_kind == kFP4) return launch_fp4_decode(L);
     if (L.kv_kind == kFP8) {
         if (D != 128) return cudaErrorInvalidValue;
         return L.io_kind == kBF16 ? launch_d<128, kFP8, kBF16>(L) : launch_d<128, kFP8, kF16>(L);

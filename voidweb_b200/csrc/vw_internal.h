@@ -74,6 +74,7 @@ struct DecodeLaunch {
 // Returns cudaSuccess or the launch error.  Unsupported shapes must have been
 // rejected by the caller.
 cudaError_t launch_paged_decode(const DecodeLaunch& L);
+cudaError_t launch_fp4_decode(const DecodeLaunch& L);    // 4-bit pools (vw_decode_fp4.cu)
 int decode_ctas_per_sm();
 size_t decode_scratch_floats_o(int grid, int head_dim);
 size_t decode_scratch_floats_ml(int grid);
