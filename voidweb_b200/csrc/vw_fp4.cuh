@@ -5,10 +5,11 @@
 // (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives; to nearest even, saturating); a
 // group whose scale rounds to 0 holds zeros.  A code stands for code * s: two
 // times four significant bits between 2^-10 and 2688, exact in f16 and in bf16,
-// so the attention multiplies codes by scales in f16 and rounds nothing.  Both
-// quotients are IEEE f32 divisions; the borders between codes are products of
-// few bits, so they fall on the side the real quotient falls on.  NaN elements
-// encode as 6 (the conversion's rule) and do not count in amax.
+// so the attention multiplies codes by scales in f16 and rounds nothing.  The
+// scale's quotient is an IEEE f32 division: the borders between E4M3 codes are
+// products of few bits, so it falls on the side the real quotient falls on.  The
+// elements' quotients: fp4_quotient.  NaN elements encode as 6 (the
+// conversion's rule) and do not count in amax.
 //
 // One page-head (16 tokens of one KV head) is one record of 18 D bytes, which one
 // bulk copy moves:
@@ -50,11 +51,26 @@ __device__ __forceinline__ float e4m3_to_f32(uint32_t code) {
     return f16_bits_to_f32(e4m3x2_to_f16x2(code) & 0xFFFFu);
 }
 
-// Four elements -> four E2M1 codes, the first in the low half of the low byte.
-__device__ __forceinline__ uint32_t fp4_encode4(const float (&v)[4], uint32_t scale_code) {
+// 1 / s of a scale code, 0 for a scale of 0 (all its elements then encode as 0).
+__device__ __forceinline__ float fp4_inverse(uint32_t scale_code) {
     const float s = e4m3_to_f32(scale_code);
-    if (s == 0.0f) return 0u;
-    const float a = __fdiv_rn(v[0], s), b = __fdiv_rn(v[1], s), c = __fdiv_rn(v[2], s), d = __fdiv_rn(v[3], s);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+    return s == 0.0f ? 0.0f : r;
+}
+
+// x / s to a multiple of 2^-13, which decides the code as the real quotient does: x * inverse is within 2^-21 of
+// x / s (relative).  A border b between codes (.25, .75, .. 5) times s has at most 7 significant bits and x at most
+// 11, so x / s is either b, and the sum rounds to b exactly (b is a multiple of .25), or off it by at least
+// 2^-11 b >= 2^-13, a whole step.  Two additions instead of a division.
+__device__ __forceinline__ float fp4_quotient(float x, float inverse) {
+    return __fsub_rn(__fadd_rn(__fmul_rn(x, inverse), 1536.0f), 1536.0f);
+}
+
+// Four elements -> four E2M1 codes, the first in the low half of the low byte.
+__device__ __forceinline__ uint32_t fp4_encode4(const float* v, float inverse) {
+    const float a = fp4_quotient(v[0], inverse), b = fp4_quotient(v[1], inverse);
+    const float c = fp4_quotient(v[2], inverse), d = fp4_quotient(v[3], inverse);
     uint16_t r;
     asm("{\n\t.reg .b8 lo, hi;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 lo, %2, %1;\n\t"
@@ -103,7 +119,7 @@ __device__ __forceinline__ void fp4_store_row(uint8_t* rec, uint8_t* rec2, int k
 #pragma unroll
     for (int off = 1; off < LANES; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
     const uint32_t sc = fp4_scale_code(amax);
-    const uint32_t codes = fp4_encode4(v, sc);
+    const uint32_t codes = fp4_encode4(v, fp4_inverse(sc));
     const int co = kv * R::V + t * R::CODE_ROW + lane * (PER / 2);
     const int g = lane / LANES;
     const int so = kv == 0 ? R::KS + t * R::GROUPS + g : R::VS + g * 16 + t;

@@ -52,31 +52,61 @@ __device__ __forceinline__ uint64_t fp4_record(const PoolGeom& g, uint32_t layer
     return (((uint64_t)layer * g.num_blocks + blk) * g.num_kv_heads + h) * Fp4Rec<D>::BYTES;
 }
 
-// The 4-bit pools' part of the append: rows w0 .. w0+3 of the launch, one row at a time.
+// Append to a 4-bit pool.  A warp takes kFp4Rows rows; a lane quantises a chunk of
+// eight elements (16 B in, a word of codes out), D/8 lanes a row, with all its
+// chunks' loads in flight first.  Two neighbouring lanes share a group's scale.
+// Instructions bound it, not bytes: one chunk is some 70.
+constexpr uint32_t kFp4Rows = 8;
+
 template <int D>
-__device__ __forceinline__ void fp4_append(const PoolGeom& g, uint8_t* data, uint32_t layer, const uint16_t* k_new,
-                                           const uint16_t* v_new, const int64_t* slots, uint32_t w0, uint32_t rows,
-                                           uint32_t lane, uint32_t* err) {
-    for (uint32_t r = 0; r < kRowsPerWarp; ++r) {
-        const uint32_t w = w0 + r;
-        if (w >= rows) return;
+__global__ void __launch_bounds__(256) fp4_append_kernel(PoolGeom g, uint8_t* __restrict__ data, uint32_t layer,
+                                                         const uint16_t* __restrict__ k_new,
+                                                         const uint16_t* __restrict__ v_new,
+                                                         const int64_t* __restrict__ slots, uint32_t n, uint32_t* err) {
+    using R = Fp4Rec<D>;
+    constexpr int WORDS = D / 8, N = kFp4Rows * WORDS / 32;      // chunks of a row, of a lane
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t w0 = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kFp4Rows;
+    const uint32_t rows = n * 2u * g.num_kv_heads;
+    uint4 raw[N];
+    uint8_t *code[N], *scale[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        raw[j] = make_uint4(0, 0, 0, 0);
+        code[j] = nullptr;
+        const uint32_t unit = j * 32 + lane, w = w0 + unit / WORDS, word = unit % WORDS;
+        if (w >= rows) continue;
         const RowIdx x = row_index(w, g.num_kv_heads);
         const int64_t slot = __ldg(slots + x.i);
         if (slot < 0) continue;
         if (slot >= (int64_t)g.num_blocks * kBlockSize) {
-            if (lane == 0) atomicOr(err, kDevErrSlot);
+            if (word == 0) atomicOr(err, kDevErrSlot);
             continue;
         }
-        const uint16_t* src = (x.kv == 0 ? k_new : v_new) + ((size_t)x.i * g.num_kv_heads + x.h) * D + lane * (D / 32);
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint16_t* src = (x.kv == 0 ? k_new : v_new) + ((size_t)x.i * g.num_kv_heads + x.h) * D;
+        raw[j] = __ldg(reinterpret_cast<const uint4*>(src) + word);
+        uint8_t* rec = data + fp4_record<D>(g, layer, (uint32_t)(slot / kBlockSize), x.h);
+        const uint32_t t = (uint32_t)(slot % kBlockSize), grp = word / 2;
+        code[j] = rec + x.kv * R::V + t * R::CODE_ROW + word * 4;
+        scale[j] = rec + (x.kv == 0 ? R::KS + t * R::GROUPS + grp : R::VS + grp * 16 + t);
+    }
 #pragma unroll
-        for (int k = 0; k < D / 64; ++k) {
-            const uint32_t two = __ldg(reinterpret_cast<const uint32_t*>(src) + k);
-            v[2 * k] = io_f32(two & 0xFFFFu, g.io_kind);
-            v[2 * k + 1] = io_f32(two >> 16, g.io_kind);
+    for (int j = 0; j < N; ++j) {
+        const uint32_t two[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+        float v[8], amax = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            v[k] = io_f32(k & 1 ? two[k / 2] >> 16 : two[k / 2] & 0xFFFFu, g.io_kind);
+            amax = fmaxf(amax, fabsf(v[k]));
         }
-        fp4_store_row<D>(data + fp4_record<D>(g, layer, (uint32_t)(slot / kBlockSize), x.h), nullptr, (int)x.kv,
-                         (int)(slot % kBlockSize), (int)lane, v);
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        const uint32_t sc = fp4_scale_code(amax);
+        const float inv = fp4_inverse(sc);
+        const uint32_t codes = fp4_encode4(v, inv) | (fp4_encode4(v + 4, inv) << 16);
+        if (code[j]) {
+            *reinterpret_cast<uint32_t*>(code[j]) = codes;
+            if ((lane & 1) == 0) *scale[j] = (uint8_t)sc;
+        }
     }
 }
 
@@ -96,11 +126,6 @@ __global__ void __launch_bounds__(256) kv_append_kernel(PoolGeom g, uint8_t* __r
     const uint32_t w0 = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kRowsPerWarp;
     const uint32_t rows = n * 2u * g.num_kv_heads;
     const uint32_t D = g.head_dim;
-    if (g.kv_kind == kFP4) {
-        if (D == 128) fp4_append<128>(g, data, layer, k_new, v_new, slots, w0, rows, lane, err);
-        else fp4_append<64>(g, data, layer, k_new, v_new, slots, w0, rows, lane, err);
-        return;
-    }
     if (g.kv_kind != kFP8) {
         // D 16-bit elements = D/4 u64 words per row: one word per lane (D 128) or
         // one per lane of the first half-warp (D 64)
@@ -202,19 +227,17 @@ __global__ void __launch_bounds__(256) block_copy_kernel(PoolGeom g, uint8_t* __
 }
 
 // Block-table gather of a 4-bit pool: the rows' values (exact) in the io type,
-// into [Hkv][seq_len][D].  A warp takes kFp4GatherRows rows; a lane expands a word
+// into [Hkv][seq_len][D].  A warp takes kFp4Rows rows; a lane expands a word
 // of eight codes, half a group, into 16 B, so D/8 lanes write a row.
-constexpr uint32_t kFp4GatherRows = 8;
-
 template <int D>
 __global__ void __launch_bounds__(256) fp4_gather_kernel(PoolGeom g, const uint8_t* __restrict__ data, uint32_t layer,
                                                          const uint32_t* __restrict__ block_table, uint32_t seq_len,
                                                          uint16_t* __restrict__ out_k, uint16_t* __restrict__ out_v,
                                                          uint32_t* err) {
     using R = Fp4Rec<D>;
-    constexpr int WORDS = D / 8, N = kFp4GatherRows * WORDS / 32;      // words of a row, words of a lane
+    constexpr int WORDS = D / 8, N = kFp4Rows * WORDS / 32;      // words of a row, words of a lane
     const uint32_t lane = threadIdx.x & 31;
-    const uint32_t w0 = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kFp4GatherRows;
+    const uint32_t w0 = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kFp4Rows;
     const uint32_t rows = seq_len * 2u * g.num_kv_heads;
     uint32_t code[N], sc[N];
     uint16_t* dst[N];
@@ -301,6 +324,13 @@ cudaError_t launch_kv_append(const PoolGeom& g, uint8_t* data, float* scales, ui
     if (n == 0) return cudaSuccess;
     const uint64_t rows = (uint64_t)n * 2 * g.num_kv_heads;
     const unsigned grid = (unsigned)((rows + 8 * kRowsPerWarp - 1) / (8 * kRowsPerWarp));
+    if (g.kv_kind == kFP4) {
+        const unsigned grid = (unsigned)((rows + 8 * kFp4Rows - 1) / (8 * kFp4Rows));
+        const uint16_t *k = static_cast<const uint16_t*>(k_new), *v = static_cast<const uint16_t*>(v_new);
+        if (g.head_dim == 128) fp4_append_kernel<128><<<grid, 256, 0, s>>>(g, data, layer, k, v, slots, n, err);
+        else fp4_append_kernel<64><<<grid, 256, 0, s>>>(g, data, layer, k, v, slots, n, err);
+        return cudaGetLastError();
+    }
     kv_append_kernel<<<grid, 256, 0, s>>>(g, data, scales, layer,
                                           static_cast<const uint16_t*>(k_new),
                                           static_cast<const uint16_t*>(v_new), slots, n, err);
@@ -322,7 +352,7 @@ cudaError_t launch_kv_gather(const PoolGeom& g, const uint8_t* data, const float
     const uint64_t rows = (uint64_t)seq_len * 2 * g.num_kv_heads;
     const unsigned grid = (unsigned)((rows + 8 * kRowsPerWarp - 1) / (8 * kRowsPerWarp));
     if (g.kv_kind == kFP4) {
-        const unsigned grid = (unsigned)((rows + 8 * kFp4GatherRows - 1) / (8 * kFp4GatherRows));
+        const unsigned grid = (unsigned)((rows + 8 * kFp4Rows - 1) / (8 * kFp4Rows));
         uint16_t *k = static_cast<uint16_t*>(out_k), *v = static_cast<uint16_t*>(out_v);
         if (g.head_dim == 128) fp4_gather_kernel<128><<<grid, 256, 0, s>>>(g, data, layer, block_table, seq_len, k, v, err);
         else fp4_gather_kernel<64><<<grid, 256, 0, s>>>(g, data, layer, block_table, seq_len, k, v, err);

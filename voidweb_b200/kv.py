@@ -11,6 +11,7 @@ on torch's current stream.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -23,12 +24,16 @@ _IO = {torch.float16: C.VW_F16, torch.bfloat16: C.VW_BF16}
 
 
 def _ptr(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else None
+    return t.data_ptr() if t is not None else None
 
 
-def _stream(stream=None):
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return ctypes.c_void_p(s.cuda_stream)
+def _stream(stream=None, device=None):
+    """The raw handle of a stream, by default torch's current one on `device` (the
+    current device).  A small decode is a few microseconds of host time, and a Stream
+    object costs two or three of them."""
+    if stream is not None:
+        return stream.cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device is None else device)
 
 
 def _window(window: int, sinks: int):
@@ -79,6 +84,7 @@ class KvPool:
                            spec.max_batch, dev.index or 0, 0,
                            _ptr(data) if data is not None else None,
                            _ptr(scales) if scales is not None else None)
+        self._index = dev.index or 0
         h = ctypes.c_void_p()
         C.check(C.lib().vw_pool_create(ctypes.byref(cfg), ctypes.byref(h)))
         self._h = h
@@ -135,16 +141,16 @@ class KvPool:
         the default, about 2 s); see vw_debug_set_wait_limit."""
         C.check(C.lib().vw_debug_set_wait_limit(self._h, cycles))
 
-    def _check(self, **tensors) -> None:
-        """Refuse a tensor the kernels would read wrongly: (tensor, shape, element bytes) per name."""
-        for name, (t, shape, size) in tensors.items():
+    def _check(self, *tensors) -> None:
+        """Refuse a tensor the kernels would read wrongly: (name, tensor, shape, element bytes) each."""
+        for name, t, shape, size in tensors:
             if t is None:
                 continue
-            if tuple(t.shape) != shape or t.element_size() != size:
+            if t.shape != shape or t.element_size() != size:
                 raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype}, expected {shape} of {size}-byte elements")
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
-            if t.device != self.device:
+            if t.get_device() != self._index:
                 raise ValueError(f"{name} is on {t.device}, the pool on {self.device}")
 
     # -- operations -------------------------------------------------------------
@@ -154,9 +160,9 @@ class KvPool:
         n = k_new.shape[0]
         if self.spec.kv_dtype == "fp4":
             row = (n, self.spec.num_kv_heads, self.spec.head_dim)
-            self._check(k_new=(k_new, row, 2), v_new=(v_new, row, 2), slot_mapping=(slot_mapping, (n,), 8))
+            self._check(("k_new", k_new, row, 2), ("v_new", v_new, row, 2), ("slot_mapping", slot_mapping, (n,), 8))
         C.check(C.lib().vw_kv_append(self._h, layer, _ptr(k_new), _ptr(v_new),
-                                     _ptr(slot_mapping), n, _stream(stream)))
+                                     _ptr(slot_mapping), n, _stream(stream, self._index)))
 
     def paged_decode(self, layer: int, q: torch.Tensor, block_tables: torch.Tensor,
                      seq_lens: torch.Tensor, out: torch.Tensor, k_new=None, v_new=None,
@@ -177,19 +183,19 @@ class KvPool:
         win = _window(window, sinks)
         if win is not None or self.spec.kv_dtype == "fp4":
             s = self.spec
-            self._check(q=(q, (B, Hq, s.head_dim), 2), out=(out, (B, Hq, s.head_dim), 2),
-                        block_tables=(block_tables, (B, block_tables.shape[-1]), 4), seq_lens=(seq_lens, (B,), 4),
-                        k_new=(k_new, (B, s.num_kv_heads, s.head_dim), 2),
-                        v_new=(v_new, (B, s.num_kv_heads, s.head_dim), 2))
+            rows, new = (B, Hq, s.head_dim), (B, s.num_kv_heads, s.head_dim)
+            self._check(("q", q, rows, 2), ("out", out, rows, 2),
+                        ("block_tables", block_tables, (B, block_tables.shape[-1]), 4),
+                        ("seq_lens", seq_lens, (B,), 4), ("k_new", k_new, new, 2), ("v_new", v_new, new, 2))
         if rope_theta > 0.0:
             flags |= C.VW_DECODE_ROPE
         a = C.DecodeArgs(layer, B, Hq, block_tables.shape[1], _ptr(q), _ptr(block_tables),
                          _ptr(seq_lens), _ptr(out), _ptr(k_new), _ptr(v_new), scale, flags,
                          rope_theta, 0)
         if win is None:
-            C.check(C.lib().vw_paged_decode(self._h, ctypes.byref(a), _stream(stream)))
+            C.check(C.lib().vw_paged_decode(self._h, ctypes.byref(a), _stream(stream, self._index)))
         else:
-            C.check(C.lib().vw_paged_decode_window(self._h, ctypes.byref(a), ctypes.byref(win), _stream(stream)))
+            C.check(C.lib().vw_paged_decode_window(self._h, ctypes.byref(a), ctypes.byref(win), _stream(stream, self._index)))
         return out
 
     def paged_prefill(self, layer: int, q: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -213,11 +219,11 @@ class KvPool:
         win = _window(window, sinks)
         if win is not None or self.spec.kv_dtype == "fp4":
             s, B = self.spec, ctx_start.shape[0]
-            self._check(q=(q, (T, Hq, s.head_dim), 2), out=(out, (T, Hq, s.head_dim), 2),
-                        cu_seqlens=(cu_seqlens, (B + 1,), 4), ctx_start=(ctx_start, (B,), 4),
-                        block_tables=(block_tables, (B, block_tables.shape[-1]), 4),
-                        k_new=(k_new, (T, s.num_kv_heads, s.head_dim), 2),
-                        v_new=(v_new, (T, s.num_kv_heads, s.head_dim), 2))
+            rows, new = (T, Hq, s.head_dim), (T, s.num_kv_heads, s.head_dim)
+            self._check(("q", q, rows, 2), ("out", out, rows, 2), ("cu_seqlens", cu_seqlens, (B + 1,), 4),
+                        ("ctx_start", ctx_start, (B,), 4),
+                        ("block_tables", block_tables, (B, block_tables.shape[-1]), 4),
+                        ("k_new", k_new, new, 2), ("v_new", v_new, new, 2))
         if causal:
             flags |= C.VW_PREFILL_CAUSAL
         if rope_theta > 0.0:
@@ -226,9 +232,9 @@ class KvPool:
                           _ptr(k_new), _ptr(v_new), _ptr(cu_seqlens), _ptr(ctx_start),
                           _ptr(block_tables), _ptr(out), scale, rope_theta)
         if win is None:
-            C.check(C.lib().vw_paged_prefill(self._h, ctypes.byref(a), _stream(stream)))
+            C.check(C.lib().vw_paged_prefill(self._h, ctypes.byref(a), _stream(stream, self._index)))
         else:
-            C.check(C.lib().vw_paged_prefill_window(self._h, ctypes.byref(a), ctypes.byref(win), _stream(stream)))
+            C.check(C.lib().vw_paged_prefill_window(self._h, ctypes.byref(a), ctypes.byref(win), _stream(stream, self._index)))
         return out
 
     def plan(self, block_tables: torch.Tensor, seq_lens: torch.Tensor, num_q_heads: int,
@@ -238,11 +244,11 @@ class KvPool:
         the next plan)."""
         C.check(C.lib().vw_decode_plan(self._h, _ptr(block_tables), _ptr(seq_lens),
                                        block_tables.shape[0], block_tables.shape[1], num_q_heads,
-                                       _stream(stream)))
+                                       _stream(stream, self._index)))
 
     def block_copy(self, pairs: torch.Tensor, stream=None) -> None:
         """Copy-on-write / compaction copy of whole blocks: pairs [n][2] (src, dst)."""
-        C.check(C.lib().vw_block_copy(self._h, _ptr(pairs), pairs.shape[0], _stream(stream)))
+        C.check(C.lib().vw_block_copy(self._h, _ptr(pairs), pairs.shape[0], _stream(stream, self._index)))
 
     def gather(self, layer: int, block_table: torch.Tensor, seq_len: int, stream=None):
         """Raw K/V rows of one sequence, [Hkv][seq_len][D] (+ FP8 scales); 4-bit
@@ -253,7 +259,13 @@ class KvPool:
             dt = torch.bfloat16 if s.io_dtype == "bf16" else torch.float16
             if block_table.dim() != 1 or block_table.shape[0] * 16 < seq_len:
                 raise ValueError(f"block_table: {tuple(block_table.shape)} for {seq_len} tokens")
-            self._check(block_table=(block_table, tuple(block_table.shape), 4))
+            self._check(("block_table", block_table, block_table.shape, 4))
+            # (the rows belong to the stream that writes them)
+            with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
+                ok, ov = (torch.empty((s.num_kv_heads, seq_len, s.head_dim), dtype=dt, device=self.device) for _ in "kv")
+            C.check(C.lib().vw_kv_gather(self._h, layer, _ptr(block_table), seq_len, _ptr(ok), _ptr(ov), None, None,
+                                         _stream(stream, self._index)))
+            return ok, ov, None, None
         ok = torch.empty((s.num_kv_heads, seq_len, s.head_dim), dtype=dt, device=self.device)
         ov = torch.empty_like(ok)
         ks = vs = None
@@ -261,7 +273,7 @@ class KvPool:
             ks = torch.empty((s.num_kv_heads, seq_len), dtype=torch.float32, device=self.device)
             vs = torch.empty_like(ks)
         C.check(C.lib().vw_kv_gather(self._h, layer, _ptr(block_table), seq_len, _ptr(ok),
-                                     _ptr(ov), _ptr(ks), _ptr(vs), _stream(stream)))
+                                     _ptr(ov), _ptr(ks), _ptr(vs), _stream(stream, self._index)))
         return ok, ov, ks, vs
 
     def decode_step_host(self, q, k_new, v_new, block_tables, seq_lens, out,
@@ -274,10 +286,10 @@ class KvPool:
         a = C.StepHostArgs(B, Hq, block_tables.shape[1], 0, _ptr(q), _ptr(k_new), _ptr(v_new),
                            _ptr(block_tables), _ptr(seq_lens), _ptr(out), scale, rope_theta)
         if win is None:
-            C.check(C.lib().vw_decode_step_host(self._h, ctypes.byref(a), _stream(stream)))
+            C.check(C.lib().vw_decode_step_host(self._h, ctypes.byref(a), _stream(stream, self._index)))
         else:
             C.check(C.lib().vw_decode_step_host_window(self._h, ctypes.byref(a), ctypes.byref(win),
-                                                       _stream(stream)))
+                                                       _stream(stream, self._index)))
 
 
 def _alias_u8(ptr: int, nbytes: int, device: torch.device) -> torch.Tensor:
