@@ -28,8 +28,8 @@
  *   scale [num_layers][num_blocks][num_kv_heads][2][16]  f32, FP8 pools only
  * 4-bit pools (VW_FP4_E2M1) have no scale buffer:
  *   data  [num_layers][num_blocks][num_kv_heads] records of 18 * head_dim bytes:
- *         K codes [16][head_dim/2], V codes [16][head_dim/2] (element 2i in the
- *         low half of byte i), K scales [16][head_dim/16], V scales
+ *         K codes [16][head_dim/2] (element 2i in the low half of byte i), K
+ *         scales [16][head_dim/16], V codes [16][head_dim/2], V scales
  *         [head_dim/16][16], the scales E4M3 bytes.  16 consecutive elements of a
  *         row share the scale s = E4M3(amax / 6); each is the E2M1 code of x / s
  *         (both to nearest even, saturating; a group whose s rounds to 0 holds

@@ -181,16 +181,22 @@ def test_prefill(kv, io, D, Hq, Hkv, chunks, window, sinks):
 
 
 @pytest.mark.parametrize("kv,io,D,Hq,Hkv", KINDS[:4] + KINDS[7:9])
-def test_prefill_whole_window_is_the_plain_prefill(kv, io, D, Hq, Hkv):
-    bt = Batch(8, kv, io, D, Hq, Hkv, [700, 40]).fill()
-    q = bt.rows(340, Hq).to(bt.dev)
-    cu = torch.tensor([0, 300, 340], dtype=torch.int32, device=bt.dev)
-    start = torch.tensor([400, 0], dtype=torch.int32, device=bt.dev)
-    a, b = torch.zeros_like(q), torch.zeros_like(q)
-    bt.pool.paged_prefill(0, q, cu, start, bt.device_table(), a)
-    bt.pool.paged_prefill(0, q, cu, start, bt.device_table(), b, window=700)
+def test_prefill_whole_window_and_long_chunks(kv, io, D, Hq, Hkv):
+    """A window of the whole context sees what a plain prefill sees; chunks of many tiles, the last rows ragged."""
+    chunks = [(400, 300), (0, 40), (1000, 777)]
+    bt = Batch(8, kv, io, D, Hq, Hkv, [a + n for a, n in chunks]).fill()
+    q = bt.rows(1117, Hq).to(bt.dev)
+    cu = torch.tensor([0, 300, 340, 1117], dtype=torch.int32, device=bt.dev)
+    start = torch.tensor([a for a, _ in chunks], dtype=torch.int32, device=bt.dev)
+    x, y = torch.zeros_like(q), torch.zeros_like(q)
+    bt.pool.paged_prefill(0, q, cu, start, bt.device_table(), x)
+    bt.pool.paged_prefill(0, q, cu, start, bt.device_table(), y, window=1777)
     assert bt.pool.check() == 0
-    assert torch.equal(a, b)
+    for b, (a, n) in enumerate(chunks):
+        r = slice(int(cu[b]), int(cu[b + 1]))
+        ref = attend(q[r].cpu(), held(bt.k[b], kv), held(bt.v[b], kv), torch.arange(a, a + n), v_scale=v_scales(bt.v[b], kv))
+        check(x[r], *ref, io, kv, f"plain {b}")
+        check(y[r], *ref, io, kv, f"window {b}")
 
 
 def test_prefill_then_decode_steps():

@@ -12,11 +12,12 @@
 // conversion's rule) and do not count in amax.
 //
 // One page-head (16 tokens of one KV head) is one record of 18 D bytes, which one
-// bulk copy moves:
-//   K codes [16][D/2], V codes [16][D/2]   element 2i in the low half of byte i
-//   K scales [16][D/16]                    a token's groups together
-//   V scales [D/16][16]                    a group's tokens together: the P V product
-//                                          pairs two tokens of one element
+// bulk copy moves, a K half and a V half:
+//   K codes [16][D/2]      element 2i in the low half of byte i
+//   K scales [16][D/16]    a token's groups together
+//   V codes [16][D/2]
+//   V scales [D/16][16]    a group's tokens together: the P V product pairs two tokens
+//                          of one element
 #pragma once
 #include <cstdint>
 
@@ -26,10 +27,11 @@ template <int D>
 struct Fp4Rec {
     static constexpr int CODE_ROW = D / 2;      // bytes of one token's codes
     static constexpr int GROUPS = D / 16;
-    static constexpr int V = 16 * CODE_ROW;     // first V code
-    static constexpr int KS = 2 * V;            // first K scale
-    static constexpr int VS = KS + 16 * GROUPS; // first V scale
-    static constexpr int BYTES = VS + 16 * GROUPS;
+    static constexpr int KS = 16 * CODE_ROW;    // first K scale
+    static constexpr int HALF = KS + 16 * GROUPS;
+    static constexpr int V = HALF;              // first V code
+    static constexpr int VS = HALF + KS;        // first V scale
+    static constexpr int BYTES = 2 * HALF;
 };
 static_assert(Fp4Rec<128>::BYTES == 2304 && Fp4Rec<64>::BYTES == 1152, "18 D bytes");
 

@@ -109,6 +109,7 @@ struct PrefillLaunch {
 
 // Returns cudaSuccess or the launch error; shapes were validated by the caller.
 cudaError_t launch_paged_prefill(const PrefillLaunch& L);
+cudaError_t launch_group_prefill(const PrefillLaunch& L);   // vw_prefill_group.cu
 int prefill_query_tile();
 
 struct PoolGeom {

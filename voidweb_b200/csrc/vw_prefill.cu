@@ -29,10 +29,9 @@
 //    memory until the epilogue.  bf16 probabilities are written as a bf16 pair
 //    hi + lo (two PV MMAs) so that P keeps ~2^-18 relative precision.
 //  * FP8 pools: decoder warps expand the codes into the same f16 tiles; the
-//    softmax applies the per-token K and V scales.  4-bit pools: they write
-//    codes times scales.
-//  * Windows: the tile visits the pages that some of its queries sees, the sinks'
-//    first (vw_window.cuh), and masks by the keys' positions.
+//    softmax applies the per-token K and V scales.  Under a window a tile visits
+//    the pages that some of its queries sees (vw_window.cuh) and masks by the
+//    keys' positions.
 //  * Every wait is bounded; on timeout the kernel records kDevErrTimeout,
 //    drains its TMA loads and returns.
 
@@ -44,12 +43,12 @@
 #include <cuda_runtime.h>
 #include <atomic>
 #include <cstdint>
-#include <type_traits>
 
+#include "vw_prefill.cuh"
+#include "vw_fp4.cuh"
 #include "vw_fp8.cuh"
 #include "vw_internal.h"
 #include "vw_ptx.cuh"
-#include "vw_fp4.cuh"
 #include "vw_rope.cuh"
 #include "vw_tc.cuh"
 #include "vw_window.cuh"
@@ -57,27 +56,6 @@
 namespace vw {
 
 namespace {
-
-constexpr int pf_align(int x, int a) { return (x + a - 1) / a * a; }
-
-template <int IO>
-__device__ __forceinline__ float pf_io_to_f32(uint32_t h) {
-    return IO == kBF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
-}
-template <int IO>
-__device__ __forceinline__ uint16_t pf_f32_to_io(float f) {
-    return IO == kBF16 ? f32_to_bf16_bits(f) : f32_to_f16_bits(f);
-}
-
-// Largest b with pfx[b] <= x over b in [0, B).
-__device__ __forceinline__ int pf_find(const int* pfx, int B, int x) {
-    int lo = 0, hi = B - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (pfx[mid] <= x) lo = mid; else hi = mid - 1;
-    }
-    return lo;
-}
 
 // Largest b in [0, B) with cu_q[b] <= i (cu_q non-decreasing, cu_q[0] <= i),
 // by the whole warp: each round the 32 lanes probe 32 evenly spaced offsets of
@@ -185,7 +163,8 @@ __global__ void __launch_bounds__(256) prefill_append_kernel(
                         const uint32_t hbits = (w2[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
                         v[e] = g.io_kind == kBF16 ? bf16_bits_to_f32(hbits) : f16_bits_to_f32(hbits);
                     }
-                    uint8_t* rec = data + (((uint64_t)layer * g.num_blocks + blk) * Hkv + h) * (18u * D);
+                    uint8_t* rec = data + (((uint64_t)layer * g.num_blocks + blk) * Hkv + h) *
+                                              page_head_bytes(kFP4, D);
                     if (D == 128) fp4_store_row<128>(rec, nullptr, (int)kv, p % kBlockSize, (int)lane, v);
                     else fp4_store_row<64>(rec, nullptr, (int)kv, p % kBlockSize, (int)lane, v);
                 } else if (g.kv_kind != kFP8) {
@@ -226,16 +205,12 @@ struct TcTraits {
     // binary16 value decode(b)/256, exact), so the MMAs run in f16 whatever the
     // io type; the factor 256 returns through the K scales and the output
     static constexpr bool FP8 = KV_ == kFP8;
-    // 4-bit pools: the decoders write code * scale, exact in f16, so nothing
-    // remains to fold
-    static constexpr bool FP4 = KV_ == kFP4;
-    static constexpr bool DEC = FP8 || FP4;           // decoder warps fill the tiles
-    static constexpr bool MBF = BF && !DEC;           // the MMAs' operand type is bf16
-    // P as a pair hi + lo of the MMA type (two PV MMAs): bf16 pages, FP8 pages,
-    // whose f16 P carries the V scales, and 4-bit pages
-    static constexpr bool PSPLIT = BF || DEC;
+    static constexpr bool MBF = BF && !FP8;           // the MMAs' operand type is bf16
+    // P as a pair hi + lo of the MMA type (two PV MMAs): bf16 pages, and FP8
+    // pages whose f16 P carries the V scales
+    static constexpr bool PSPLIT = BF || FP8;
     static constexpr float VFOLD = FP8 ? 256.0f : 1.0f;
-    static constexpr int NDEC = DEC ? 2 : 0;          // decoder warps (FP8 and 4-bit pools)
+    static constexpr int NDEC = FP8 ? 2 : 0;          // decoder warps (FP8 pools)
     static constexpr int CH = D * 2 / 128;            // 128-B columns of a row
     static constexpr int R = kTcPages;                // page-heads per round
     static constexpr int KEYS = 16 * R;               // keys per round: the N of S = Q K^T
@@ -246,7 +221,7 @@ struct TcTraits {
     // 128 the K ring is one deeper, which is what shared memory holds with two
     // CTAs per SM (what tensor memory allows); head_dim 64 keeps 4 + 4.
     static constexpr int NST = D == 128 ? 2 : 4;
-    static constexpr int NSTK = (D == 128 && !DEC) ? 3 : NST;
+    static constexpr int NSTK = (D == 128 && !FP8) ? 3 : NST;
     static constexpr int NSTV = NST;
     static constexpr int TILE = CH * KEYS * 128;      // bytes of one K (or V) tile
     static constexpr int HALF_BOX = 16 * 128;         // one TMA box: 16 rows of one column
@@ -270,13 +245,13 @@ struct TcTraits {
     static constexpr int SMEM = QBYTES + (NSTK + NSTV) * TILE + SCL + NBAR * 8 + 16;
     // 4 softmax warps, 1 MMA warp, then 2 TMA producer warps (K tiles, V tiles)
     // or NDEC decoder warps
-    static constexpr int THREADS = (DEC ? 5 + NDEC : 7) * 32;
+    static constexpr int THREADS = (FP8 ? 5 + NDEC : 7) * 32;
     static constexpr uint32_t IDESC_S = idesc_f16(MBF, false, kTcRows, KEYS);
     static constexpr uint32_t IDESC_PV = idesc_f16(MBF, true, kTcRows, D);
     static_assert(D == 64 || D == 128, "head_dim 64 or 128");
     static_assert(!FP8 || D == 128, "FP8 pools have head_dim 128");
     static_assert(!FP8 || NDEC * 32 == KEYS, "one decoder thread per key of a round (scales)");
-    static_assert(!DEC || NSTK == NSTV, "decoders fill a round's K and V tiles together");
+    static_assert(!FP8 || NSTK == NSTV, "FP8 decoders fill a round's K and V tiles together");
     static_assert(TPFX <= TILE, "the tile prefix fits in a V tile");
     static_assert(COL_S + 2 * KEYS <= (int)TMEM_COLS, "tensor-memory columns");
     static_assert(QBYTES % 1024 == 0 && TILE % 1024 == 0, "1024-B alignment");
@@ -300,7 +275,6 @@ struct Fp8RoundRegs {
     float ks, vs;
 };
 
-// (FP8 and 4-bit pools)
 template <class T, bool WIN>
 __device__ __forceinline__ void fp8_round_ids(const uint32_t* bt, int t, int npages, const PageSpan& sp,
                                               uint32_t (&blk)[T::R]) {
@@ -356,84 +330,6 @@ __device__ __forceinline__ void fp8_store_round(uint8_t* kt, uint8_t* vt, float*
                                     fp8x2_to_f16x2_scaled(r.w[i].w, 0), fp8x2_to_f16x2_scaled(r.w[i].w, 1));
         *reinterpret_cast<uint4*>(row + ((ua ^ (key & 7)) << 4)) = a;
         *reinterpret_cast<uint4*>(row + (((ua + 1) ^ (key & 7)) << 4)) = bq;
-    }
-    // generic-proxy writes, read next by the tensor cores (async proxy)
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
-// 4-bit pools: the decoders' part of a round.  A chunk is 16 B, 32 codes of one
-// row, with the scales of its two groups; a thread's chunks lie at one place of
-// their page-heads (unit u of row rr), page-heads PPI apart, so a warp reads whole
-// runs of a record.  Codes and scales multiply to exact f16 values, which go to the
-// same tiles as an f16 pool's rows.
-template <class T>
-struct Fp4Round {
-    static constexpr int U = T::D / 32;                       // chunks of a row
-    static constexpr int THR = 16 * U;                        // threads of a page-head
-    static constexpr int PPI = T::NDEC * 32 / THR;            // page-heads at once
-    static constexpr int N = T::R / PPI;                      // chunks per thread and half (K, V)
-    static_assert(T::NDEC * 32 % THR == 0 && T::R % PPI == 0, "decoder threads cover whole page-heads");
-    uint4 w[2][N];
-    uint32_t sc[2][N];                                        // the two groups' E4M3 codes
-};
-
-template <class T, bool WIN>
-__device__ __forceinline__ void fp4_load_round(const PrefillParams& p, const uint32_t (&blk)[T::R], int t, int h,
-                                               int total, int npages, const PageSpan& sp, int dt, Fp4Round<T>& r) {
-    using Q = Fp4Round<T>;
-    using Rec = Fp4Rec<T::D>;
-    if (dt == 0)
-#pragma unroll
-        for (int pg = 0; pg < T::R; ++pg)
-            if (t * T::R + pg < npages && blk[pg] >= p.num_blocks) atomicOr(p.err, kDevErrBlockId);
-    const int u = dt % Q::U, rr = dt / Q::U % 16;
-#pragma unroll
-    for (int i = 0; i < Q::N; ++i) {
-        uint32_t b = 0xFFFFFFFFu;
-        int pg = 0;
-#pragma unroll
-        for (int k = 0; k < Q::PPI; ++k)
-            if (dt / Q::THR == k) { b = blk[i * Q::PPI + k]; pg = i * Q::PPI + k; }
-        const int o = t * T::R + pg, pos = (WIN ? sp.page(o) : o) * kBlockSize + rr;
-        const bool valid = b < p.num_blocks && pos < total && (!WIN || pos < sp.sinks || pos >= sp.lo);
-        const uint8_t* rec = p.kv_data + (((size_t)p.layer * p.num_blocks + b) * p.Hkv + (uint32_t)h) * Rec::BYTES;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            r.w[kv][i] = make_uint4(0, 0, 0, 0);
-            r.sc[kv][i] = 0;
-        }
-        if (valid) {
-            r.w[0][i] = __ldg(reinterpret_cast<const uint4*>(rec + rr * Rec::CODE_ROW + u * 16));
-            r.w[1][i] = __ldg(reinterpret_cast<const uint4*>(rec + Rec::V + rr * Rec::CODE_ROW + u * 16));
-            r.sc[0][i] = __ldg(reinterpret_cast<const uint16_t*>(rec + Rec::KS + rr * Rec::GROUPS + 2 * u));
-            r.sc[1][i] = __ldg(rec + Rec::VS + 32 * u + rr) | ((uint32_t)__ldg(rec + Rec::VS + 32 * u + 16 + rr) << 8);
-        }
-    }
-}
-
-template <class T>
-__device__ __forceinline__ void fp4_store_round(uint8_t* kt, uint8_t* vt, int dt, const Fp4Round<T>& r) {
-    using Q = Fp4Round<T>;
-    const int u = dt % Q::U, rr = dt / Q::U % 16;
-    const int c = u >> 1, ua = (u & 1) * 4;                   // 128-B column, first 16-B unit
-#pragma unroll
-    for (int i = 0; i < Q::N; ++i) {
-        const int key = (i * Q::PPI + dt / Q::THR) * 16 + rr;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            uint8_t* row = (kv ? vt : kt) + c * (T::KEYS * 128) + key * 128;
-            const uint32_t s = e4m3x2_to_f16x2(r.sc[kv][i]);
-            const uint32_t s0 = __byte_perm(s, s, 0x1010u), s1 = __byte_perm(s, s, 0x3232u);
-            const uint32_t w[4] = {r.w[kv][i].x, r.w[kv][i].y, r.w[kv][i].z, r.w[kv][i].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                uint32_t f[4];
-                fp4x8_to_f16(w[k], f);
-                const uint32_t m = k < 2 ? s0 : s1;
-                *reinterpret_cast<uint4*>(row + (((ua + k) ^ (key & 7)) << 4)) =
-                    make_uint4(f16x2_mul(f[0], m), f16x2_mul(f[1], m), f16x2_mul(f[2], m), f16x2_mul(f[3], m));
-            }
-        }
     }
     // generic-proxy writes, read next by the tensor cores (async proxy)
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -496,11 +392,11 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < T::NSTK; ++s) {
-            mbar_init(&full_k[s], T::DEC ? T::NDEC : 1);  // decoder warps, or the TMA transaction
+            mbar_init(&full_k[s], T::FP8 ? T::NDEC : 1);  // decoder warps, or the TMA transaction
             mbar_init(&empty_k[s], 1);
         }
         for (int s = 0; s < T::NSTV; ++s) {
-            mbar_init(&full_v[s], T::DEC ? T::NDEC : 1);
+            mbar_init(&full_v[s], T::FP8 ? T::NDEC : 1);
             mbar_init(&empty_v[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -596,7 +492,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
                 lo = make_uint4(a[0], a[1], a[2], a[3]);
                 hi = make_uint4(c[0], c[1], c[2], c[3]);
             }
-            if constexpr (T::DEC && T::BF) {           // FP8 and 4-bit pages compute in f16
+            if constexpr (T::FP8 && T::BF) {           // FP8 pages compute in f16
                 auto cv = [](uint32_t x) {
                     return pack2<false>(bf16_bits_to_f32(x & 0xFFFFu), bf16_bits_to_f32(x >> 16));
                 };
@@ -615,7 +511,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
     tc_fence_after();
     const uint32_t tbase = *tmem_slot;
 
-    if (T::DEC && warp >= 5) {
+    if (T::FP8 && warp >= 5) {
         // ---- decoders: round t into stage t % NST
         const int dt = threadIdx.x - 5 * 32;
         const uint32_t* bt = p.block_tables + (size_t)b * p.bt_stride;
@@ -628,10 +524,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
 #pragma unroll
             for (int pg = 0; pg < T::R; ++pg) blk[pg] = nblk[pg];
             Fp8RoundRegs r;
-            std::conditional_t<T::FP4, Fp4Round<T>, int> r4;
-            // in flight during the wait
-            if constexpr (T::FP4) fp4_load_round<T, WIN>(p, blk, t, h, total, npages, span, dt, r4);
-            else if constexpr (T::FP8) fp8_load_round<T, WIN>(p, blk, t, h, total, npages, span, dt, r);
+            fp8_load_round<T, WIN>(p, blk, t, h, total, npages, span, dt, r);   // in flight during the wait
             fp8_round_ids<T, WIN>(bt, t + 1, npages, span, nblk);
             // the V tile's release follows the K tile's (P V is committed after S)
             if (t >= T::NST &&
@@ -639,9 +532,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
                 ok = false;
                 break;
             }
-            uint8_t *kt = ktiles + st_i * T::TILE, *vt = vtiles + st_i * T::TILE;
-            if constexpr (T::FP4) fp4_store_round<T>(kt, vt, dt, r4);
-            else if constexpr (T::FP8) fp8_store_round<T>(kt, vt, scl + st_i * 2 * T::KEYS, dt, r);
+            fp8_store_round<T>(ktiles + st_i * T::TILE, vtiles + st_i * T::TILE, scl + st_i * 2 * T::KEYS, dt, r);
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&full_k[st_i]);
@@ -731,31 +622,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
                 const int bb = t & 1, st_i = t % T::NSTV;
                 if (!mbar_wait(&p_full[bb], (t >> 1) & 1, deadline)) return false;
                 if (!mbar_wait(&full_v[st_i], (t / T::NSTV) & 1, deadline)) return false;
-                const int keyl = WIN ? 0 : total - t * T::KEYS;   // keys of the round inside the sequence
-                if constexpr (WIN && !T::DEC) {
-                    // V rows that no query of the tile sees, outside the window or
-                    // past the sequence's end: zeroed, as below, in the few pages
-                    // that hold some
-                    uint8_t* vt = vtiles + st_i * T::TILE;
-                    bool wrote = false;
-                    for (int pg = 0; pg < T::R && t * T::R + pg < npages; ++pg) {
-                        const int lp = span.page(t * T::R + pg);
-                        int a, z;
-                        span.hidden(lp, a, z);
-                        const int endr = total - lp * kBlockSize;
-                        if (a >= z && endr >= kBlockSize) continue;
-                        wrote = true;
-                        for (int row = 0; row < kBlockSize; ++row) {
-                            if (!(row >= a && row < z) && row < endr) continue;
-                            for (int c = 0; c < T::CH; ++c)
-                                for (int u = 0; u < 8; ++u)
-                                    *reinterpret_cast<uint4*>(vt + c * (T::KEYS * 128) + (pg * kBlockSize + row) * 128 +
-                                                              u * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                    }
-                    if (wrote) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
-                if (!T::DEC && keyl < T::KEYS && keyl > 0 && (keyl & 15)) {
+                const int keyl = total - t * T::KEYS;   // keys of the round inside the sequence
+                if (!T::FP8 && keyl < T::KEYS && keyl > 0 && (keyl & 15)) {
                     // the page-head holding the sequence's last key: its V rows past
                     // the end hold whatever the pool has there; zero them so that
                     // masked probabilities cannot meet NaN or Inf
@@ -914,8 +782,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) 
                     const float p0 = ex2(fmaf(xs[16 * c8 + 2 * k], p.scale_log2, -mu));
                     const float p1 = ex2(fmaf(xs[16 * c8 + 2 * k + 1], p.scale_log2, -mu));
                     ls += p0 + p1;
-                    if constexpr (T::DEC) {
-                        const float a0 = T::FP8 ? p0 * vsc[2 * k] : p0, a1 = T::FP8 ? p1 * vsc[2 * k + 1] : p1;
+                    if constexpr (T::FP8) {
+                        const float a0 = p0 * vsc[2 * k], a1 = p1 * vsc[2 * k + 1];
                         ph[k] = pack2<false>(a0, a1);
                         pl[k] = pack2<false>(a0 - f16_bits_to_f32(ph[k] & 0xFFFFu), a1 - f16_bits_to_f32(ph[k] >> 16));
                     } else {
@@ -998,10 +866,14 @@ cudaError_t launch_w(const PrefillLaunch& L) {
     return cudaLaunchKernelEx(&cfg, prefill_kernel<T, WIN>, *L.tmap, p);
 }
 
-// (the windowed kernels are instances of their own, as in the decode)
+// Windows: FP8 pools have an instance of their own here, the others the grouped kernel
+// (vw_prefill_group.cu).
 template <class T>
 cudaError_t launch_t(const PrefillLaunch& L) {
-    return L.p.window > 0 ? launch_w<T, true>(L) : launch_w<T, false>(L);
+    if constexpr (T::FP8) {
+        if (L.p.window > 0) return launch_w<T, true>(L);
+    }
+    return launch_w<T, false>(L);
 }
 
 }  // namespace
@@ -1009,11 +881,8 @@ cudaError_t launch_t(const PrefillLaunch& L) {
 int prefill_query_tile() { return kTcRows; }
 
 cudaError_t launch_paged_prefill(const PrefillLaunch& L) {
-    if (L.kv_kind == kFP4) {
-        if (L.head_dim == 64)
-            return L.io_kind == kBF16 ? launch_t<TcTraits<64, kBF16, kFP4>>(L) : launch_t<TcTraits<64, kF16, kFP4>>(L);
-        return L.io_kind == kBF16 ? launch_t<TcTraits<128, kBF16, kFP4>>(L) : launch_t<TcTraits<128, kF16, kFP4>>(L);
-    }
+    // 4-bit pools, and f16 / bf16 pools under a window
+    if (L.kv_kind == kFP4 || (L.p.window > 0 && L.kv_kind != kFP8)) return launch_group_prefill(L);
     if (L.kv_kind == kFP8) {
         if (L.head_dim != 128) return cudaErrorNotSupported;
         return L.io_kind == kBF16 ? launch_t<TcTraits<128, kBF16, kFP8>>(L)

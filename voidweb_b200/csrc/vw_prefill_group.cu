@@ -1,0 +1,669 @@
+// vw_prefill_group.cu -- the prefill attention of 4-bit pools, and of f16 / bf16 pools under a
+// window.
+//
+//  * Work split.  The query heads of a KV head are taken together: row r of a
+//    (sequence, KV head) is query head r % group of chunk token r / group, and a CTA takes
+//    128 consecutive rows, the M of the matrix instructions.  A CTA so spans few
+//    tokens (19 with 7 query heads), which visit hardly more keys than one of them
+//    does, and a short chunk still fills its tile.
+//  * Rounds of 64 keys, as in vw_prefill.cu: S = Q K^T into one of two S buffers in
+//    tensor memory while the softmax works on the other, P over S, O += P V; two
+//    CTAs per SM.  (Rounds of 128 keys leave tensor memory for one S per tile: S,
+//    softmax and P V then follow one another, and measured slower with one tile
+//    per CTA and two CTAs, 5757 cycles per 128 keys and SM against 4033, and with two tiles
+//    per CTA, 4593.)
+//  * Warps 0-3: softmax, one row per thread.  Warp 4 issues the matrix instructions.
+//    f16 / bf16 pages: warp 5 streams K tiles, warp 6 V tiles (TMA).  4-bit pages:
+//    warp 5 copies the records' K halves into a ring and expands them into f16
+//    tiles, warp 6 the V halves.
+//  * bf16 probabilities are a pair hi + lo (two P V products, as in vw_prefill.cu),
+//    those of f16 and 4-bit pages one f16.
+//  * Every wait is bounded; on timeout the kernel records kDevErrTimeout, waits
+//    for its copies and matrix instructions in flight and returns.
+#define VW_MBAR_SUSPEND_HINT_NS 0
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <atomic>
+#include <cstdint>
+
+#include "vw_prefill.cuh"
+#include "vw_fp4.cuh"
+#include "vw_rope.cuh"
+#include "vw_tc.cuh"
+#include "vw_window.cuh"
+
+namespace vw {
+
+namespace {
+
+constexpr int kGRows = 128;                       // query rows per CTA
+constexpr int kGKeys = 64;                        // keys per round
+constexpr int kGPages = kGKeys / kBlockSize;
+constexpr float kGRescale = 8.0f;                 // log2 units: p <= 2^8 against a stale max
+
+template <int D_, int IO_, int KV_>
+struct Grp {
+    static constexpr int D = D_, IO = IO_;
+    static constexpr bool FP4 = KV_ == kFP4;
+    static constexpr bool MBF = IO == kBF16 && !FP4;          // the matrix instructions' type is bf16
+    static constexpr bool PSPLIT = MBF;
+    static constexpr int CH = D * 2 / 128;                    // 128-B columns of a row
+    static constexpr int QTILE = CH * 128 * 128;              // [CH][128 rows][128 B]
+    static constexpr int TILE = CH * kGKeys * 128;            // one K or V tile
+    // K tiles and V tiles: a K tile frees when S of its round completes, rounds before the V
+    // tile of that round, so where shared memory allows the K ring is one deeper
+    static constexpr int NSTK = D == 64 ? 4 : FP4 ? 2 : 3;
+    static constexpr int NSTV = D == 64 ? 4 : 2;
+    // 4-bit record halves in the ring of the K decoder, and of the V decoder
+    static constexpr int HALF = FP4 ? Fp4Rec<D>::HALF : 0;
+    static constexpr int SLOTS = FP4 ? 7 * (128 / D) : 0;
+    static constexpr int KSTEPS = D / 16;
+    static constexpr int COL_S = D;                           // O in columns [0, D), two S buffers after it
+    // full, empty of K and V tiles; s_full, p_full, p_free of both buffers; q_full, landed, done; raw rings
+    static constexpr int NBAR = 2 * NSTK + 2 * NSTV + 9 + 2 * SLOTS;
+    static constexpr int TPFX = pf_align((kMaxBatchPerLaunch + 1) * 4, 128);
+    static constexpr int SMEM = QTILE + (NSTK + NSTV) * TILE + 2 * SLOTS * HALF + NBAR * 8 + 16;
+    static constexpr int THREADS = 7 * 32;
+    static constexpr uint32_t IDESC_S = idesc_f16(MBF, false, 128, kGKeys);
+    static constexpr uint32_t IDESC_PV = idesc_f16(MBF, true, 128, D);
+    static_assert(COL_S + 2 * kGKeys <= 256, "tensor-memory columns");
+    static_assert(2 * (SMEM + 1024) <= 233472, "two CTAs per SM");
+    static_assert(3 * (SMEM + 1024) > 233472, "at most two CTAs per SM (tensor memory)");
+    static_assert(TPFX <= TILE, "the tile prefix fits in a V tile");
+    static_assert(HALF % 16 == 0 && SLOTS < 32, "ring slots: 16-B aligned, issued within a batch of ids");
+};
+
+template <class T, bool WIN>
+__global__ void __launch_bounds__(T::THREADS, 2)
+prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    // the 128-B-swizzled tiles need 1024-B alignment; the layout has no slack
+    if (smem_u32(smem_raw) & 1023u) {
+        if (threadIdx.x == 0) atomicOr(p.err, kDevErrLaunch);
+        return;
+    }
+    uint8_t* qs = smem_raw;
+    uint8_t* ktiles = qs + T::QTILE;
+    uint8_t* vtiles = ktiles + T::NSTK * T::TILE;
+    uint8_t* raw = vtiles + T::NSTV * T::TILE;          // 4-bit records
+    int* tpfx = reinterpret_cast<int*>(vtiles + (T::NSTV - 1) * T::TILE);   // prologue only
+    uint64_t* full_k = reinterpret_cast<uint64_t*>(raw + 2 * T::SLOTS * T::HALF);
+    uint64_t* empty_k = full_k + T::NSTK;
+    uint64_t* full_v = empty_k + T::NSTK;
+    uint64_t* empty_v = full_v + T::NSTV;
+    uint64_t* s_full = empty_v + T::NSTV;
+    uint64_t* p_full = s_full + 2;
+    uint64_t* p_free = p_full + 2;
+    uint64_t* q_full = p_free + 2;
+    uint64_t* landed = q_full + 1;
+    uint64_t* done = landed + 1;
+    uint64_t* full_r = done + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full_r + 2 * T::SLOTS);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t deadline = cycles() + (p.wait_cycles ? p.wait_cycles : kWaitDeadlineCycles);
+    // test hook (vw_debug_set_wait_limit): no K/V tile is filled
+    const bool withhold = p.wait_cycles != 0;
+
+    if (threadIdx.x == 0) {
+        // (full: the decoder, or the TMA transaction)
+        for (int s = 0; s < T::NSTK; ++s) { mbar_init(&full_k[s], 1); mbar_init(&empty_k[s], 1); }
+        for (int s = 0; s < T::NSTV; ++s) { mbar_init(&full_v[s], 1); mbar_init(&empty_v[s], 1); }
+        for (int c = 0; c < 2; ++c) { mbar_init(&s_full[c], 1); mbar_init(&p_full[c], 4); mbar_init(&p_free[c], 1); }
+        mbar_init(q_full, 4);
+        mbar_init(landed, 1);
+        mbar_init(done, 1);
+        for (int s = 0; s < 2 * T::SLOTS; ++s) mbar_init(&full_r[s], 1);
+        fence_mbar_init();
+    }
+    if (p.flags & kDecodePdl) griddep_wait();          // q, chunk rows and pages from the predecessor
+    const int g = (int)p.group;
+    // CTAs per sequence and KV head, prefix over the batch (warp 0)
+    if (warp == 0) {
+        int run = 0;
+        if (lane == 0) tpfx[0] = 0;
+        for (int b0 = 0; b0 < (int)p.B; b0 += 32) {
+            const int b = b0 + lane;
+            int nt = 0;
+            if (b < (int)p.B) {
+                const int n = __ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b);
+                // (a chunk past q's T rows is refused below)
+                nt = n > 0 ? (int)(((long long)min(n, (int)p.T) * g + kGRows - 1) / kGRows) : 0;
+            }
+            int incl = nt;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, off);
+                if (lane >= off) incl += v;
+            }
+            if (b < (int)p.B) tpfx[b + 1] = run + incl;
+            run += __shfl_sync(0xffffffffu, incl, 31);
+        }
+    }
+    __syncthreads();
+    // the last CTAs of a causal chunk visit the most keys: they start first
+    // (more CTAs than the grid: chunk offsets that are not those of T rows)
+    if (tpfx[p.B] > (int)gridDim.x && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(p.err, kDevErrSeqLen);
+    const int x = tpfx[p.B] - 1 - (int)blockIdx.x;
+    if (x < 0) return;
+    const int b = pf_find(tpfx, (int)p.B, x);
+    const int row0 = (x - tpfx[b]) * kGRows;           // first row of the CTA in its (sequence, KV head)
+    const int q_off = __ldg(p.cu_q + b);
+    const int n = __ldg(p.cu_q + b + 1) - q_off;
+    const int cs = __ldg(p.ctx_start + b);
+    const int total = cs + n;
+    // the offsets come from device memory: a chunk outside q's T rows or past
+    // its block-table row is flagged and skipped
+    if (q_off < 0 || q_off + n > (int)p.T || cs < 0 || total > (int)(p.bt_stride * kBlockSize)) {
+        if (threadIdx.x == 0) atomicOr(p.err, kDevErrSeqLen);
+        return;
+    }
+    const int h = blockIdx.y, rows = n * g;
+    const int tok0 = row0 / g, tok1 = (min(row0 + kGRows, rows) - 1) / g;
+    const int kend = p.causal ? cs + tok1 + 1 : total; // keys [0, kend)
+    int npages = (kend + kBlockSize - 1) / kBlockSize; // pages visited (ordinals, mapped by span.page)
+    PageSpan span{};
+    if constexpr (WIN) {
+        span = page_span(npages, cs + tok0, p.window, p.sinks);
+        npages = span.n;
+    }
+    const int nrounds = (npages + kGPages - 1) / kGPages;
+    const uint32_t* bt = p.block_tables + (size_t)b * p.bt_stride;
+    auto page_of = [&](int o) { return WIN ? span.page(o) : o; };
+    auto id_of = [&](int o) { return o < npages ? __ldg(bt + page_of(o)) : 0xFFFFFFFFu; };
+
+    if (warp == 4) {
+        tmem_alloc(tmem_slot, 256);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();                                   // tensor memory, and the prefix is read by all
+    tc_fence_after();
+    const uint32_t tbase = *tmem_slot;
+
+    if (warp < 4) {
+        // ---- softmax: thread r owns query row row0 + r
+        const int r = threadIdx.x, row = row0 + r;
+        const bool live = row < rows;
+        const int tq = live ? row / g : 0;
+        const size_t qrow = (size_t)(q_off + tq) * p.Hq + (size_t)h * g + (live ? row - tq * g : 0);
+        {
+            // the query row into the swizzled K-major tile: 16-B unit u goes to column
+            // u / 8, unit (u % 8) ^ (r % 8); rotated first with rope_theta > 0
+            const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q) + qrow * T::D * 2;
+            constexpr int U = T::D / 8, HALF = U / 2;
+#pragma unroll
+            for (int u = 0; u < HALF; ++u) {
+                uint4 lo = make_uint4(0, 0, 0, 0), hi = make_uint4(0, 0, 0, 0);
+                if (live) {
+                    lo = __ldg(reinterpret_cast<const uint4*>(src + u * 16));
+                    hi = __ldg(reinterpret_cast<const uint4*>(src + (u + HALF) * 16));
+                }
+                uint32_t e[4] = {lo.x, lo.y, lo.z, lo.w}, f[4] = {hi.x, hi.y, hi.z, hi.w};
+                if (p.rope_theta > 0.0f && live) {
+                    // pairs (d, d + D/2): element of unit u with that of unit u + D/16
+                    const float pos = (float)(cs + tq);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        float ar = pf_io_to_f32<T::IO>(e[w] & 0xFFFFu), ai = pf_io_to_f32<T::IO>(f[w] & 0xFFFFu);
+                        float br = pf_io_to_f32<T::IO>(e[w] >> 16), bi = pf_io_to_f32<T::IO>(f[w] >> 16);
+                        const int d = u * 8 + 2 * w;
+                        rope_pair(ar, ai, d, T::D, p.rope_theta, pos);
+                        rope_pair(br, bi, d + 1, T::D, p.rope_theta, pos);
+                        e[w] = (uint32_t)pf_f32_to_io<T::IO>(ar) | ((uint32_t)pf_f32_to_io<T::IO>(br) << 16);
+                        f[w] = (uint32_t)pf_f32_to_io<T::IO>(ai) | ((uint32_t)pf_f32_to_io<T::IO>(bi) << 16);
+                    }
+                }
+                if constexpr (T::FP4 && T::IO == kBF16) {          // 4-bit pages compute in f16
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        e[w] = pack2<false>(bf16_bits_to_f32(e[w] & 0xFFFFu), bf16_bits_to_f32(e[w] >> 16));
+                        f[w] = pack2<false>(bf16_bits_to_f32(f[w] & 0xFFFFu), bf16_bits_to_f32(f[w] >> 16));
+                    }
+                }
+                const int u2 = u + HALF;
+                *reinterpret_cast<uint4*>(qs + (u >> 3) * 16384 + r * 128 + (((u & 7) ^ (r & 7)) << 4)) =
+                    make_uint4(e[0], e[1], e[2], e[3]);
+                *reinterpret_cast<uint4*>(qs + (u2 >> 3) * 16384 + r * 128 + (((u2 & 7) ^ (r & 7)) << 4)) =
+                    make_uint4(f[0], f[1], f[2], f[3]);
+            }
+            // generic-proxy writes, read next by the tensor cores (async proxy)
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        {
+            const int kend_r = live ? (p.causal ? cs + tq + 1 : total) : 0;
+            const int lo_r = WIN ? max(0, kend_r - (int)p.window) : 0;      // first key of the row's window
+            const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+            const uint32_t ocol = tbase + lanes;
+            float m_ref = -INFINITY, l = 0.0f;
+            bool ok = true;
+            for (int t = 0; t < nrounds; ++t) {
+                const int bb = t & 1;
+                const uint32_t scol = tbase + lanes + T::COL_S + bb * kGKeys;
+                if (!__all_sync(0xffffffffu, mbar_wait(&s_full[bb], (t >> 1) & 1, deadline))) { ok = false; break; }
+                tc_fence_after();
+                float xs[kGKeys];
+                tmem_ld32f(scol, xs);
+                tmem_ld32f(scol + 32, xs + 32);
+                tmem_wait_ld();
+                // does the row see every key of the round?  (a round of sink pages and
+                // window pages is taken key by key)
+                const int f = page_of(t * kGPages) * kBlockSize, e = page_of(t * kGPages + kGPages - 1) * kBlockSize;
+                bool whole = e + kBlockSize <= kend_r;
+                if constexpr (WIN)
+                    whole = whole && e - f == (kGPages - 1) * kBlockSize && (f >= lo_r || e + kBlockSize <= span.sinks);
+                if (!__all_sync(0xffffffffu, whole)) {
+                    // keys of page-heads past npages are stale rows; they lie past kend_r
+#pragma unroll
+                    for (int k = 0; k < kGKeys; ++k) {
+                        const int pos = page_of(t * kGPages + k / kBlockSize) * kBlockSize + k % kBlockSize;
+                        xs[k] = pos < kend_r && (!WIN || pos >= lo_r || pos < span.sinks) ? xs[k] : -INFINITY;
+                    }
+                }
+                // Scores stay unscaled (scale > 0 keeps the order); the scale is folded into
+                // the exponent below.  Four chains of maxima, not one of 64 steps.
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int k = 0; k < kGKeys; k += 8)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) m4[c] = fmax3(m4[c], xs[k + 2 * c], xs[k + 2 * c + 1]);
+                const float tmax = fmaxf(fmax3(m4[0], m4[1], m4[2]), m4[3]) * p.scale_log2;
+                const bool need = tmax > m_ref + kGRescale;
+                float alpha = 1.0f;
+                if (need) {
+                    alpha = ex2(m_ref - tmax);      // 0 while the row had no key
+                    m_ref = tmax;
+                }
+                if (__any_sync(0xffffffffu, need && t > 0)) {
+                    // rescale O: after P V of the round before (whose phase is the next of its
+                    // buffer: S of this round was issued after P V two rounds before completed)
+                    if (!__all_sync(0xffffffffu, mbar_wait(&p_free[bb ^ 1], ((t - 1) >> 1) & 1, deadline))) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c0 = 0; c0 < T::D; c0 += 16) {
+                        uint32_t o16[16];
+                        tmem_ld16(ocol + c0, o16);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) o16[k] = __float_as_uint(__uint_as_float(o16[k]) * alpha);
+                        tmem_st16(ocol + c0, o16);
+                    }
+                }
+                l *= alpha;
+                const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
+                const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), mu2 = make_float2(-mu, -mu);
+                float2 ls[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                // P over S: 32 keys take 16 columns of hi (or of the one f16) and, with a pair,
+                // 16 of lo
+#pragma unroll
+                for (int c = 0; c < kGKeys / 32; ++c) {
+                    uint32_t ph[16], pl[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float2 ev = fma2(make_float2(xs[32 * c + 2 * k], xs[32 * c + 2 * k + 1]), sc2, mu2);
+                        const float2 pr = make_float2(ex2(ev.x), ex2(ev.y));
+                        ls[k & 1] = add2(ls[k & 1], pr);
+                        ph[k] = pack2<T::MBF>(pr.x, pr.y);
+                        if constexpr (T::PSPLIT) {
+                            // hi as a negative pair, then lo = p - hi
+                            const float2 hi = make_float2(__uint_as_float((ph[k] << 16) ^ 0x80000000u),
+                                                          __uint_as_float((ph[k] & 0xFFFF0000u) ^ 0x80000000u));
+                            const float2 lo = add2(pr, hi);
+                            pl[k] = pack2<true>(lo.x, lo.y);
+                        }
+                    }
+                    tmem_st16(scol + 32 * c, ph);
+                    if constexpr (T::PSPLIT) tmem_st16(scol + 32 * c + 16, pl);
+                }
+                l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[bb]);
+            }
+            // epilogue: O / l, after the last P V
+            if (ok && __all_sync(0xffffffffu, mbar_wait(done, 0, deadline))) {
+                tc_fence_after();
+                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + qrow * T::D * 2;
+#pragma unroll 1
+                for (int c0 = 0; c0 < T::D; c0 += 32) {
+                    float o[32];
+                    tmem_ld32f(ocol + c0, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            w[k] = (uint32_t)pf_f32_to_io<T::IO>(o[8 * u + 2 * k] * inv) |
+                                   ((uint32_t)pf_f32_to_io<T::IO>(o[8 * u + 2 * k + 1] * inv) << 16);
+                        if (live) *reinterpret_cast<uint4*>(dst + c0 * 2 + 16 * u) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            } else if (lane == 0) {
+                atomicOr(p.err, kDevErrTimeout);
+            }
+        }
+    } else if (warp == 4) {
+        // ---- MMA issuer: the warp runs as one, lane 0 issues
+        const uint32_t on = lane == 0;
+        // descriptors: bases to which a k-step adds (kk / 4) * column + (kk % 4) * 32 bytes
+        // (>> 4 in the address field, which never carries: shared memory ends below
+        // 256 KB).  K tile: K-major, 8-key groups 1024 B apart; V tile: MN-major, 64-element
+        // columns 8 KB apart, 8-key groups 1024 B apart.
+        const uint64_t qdesc = smem_desc_sw128(smem_u32(qs), 16, 1024);
+        const uint64_t kdesc = smem_desc_sw128(smem_u32(ktiles), 16, 1024);
+        const uint64_t vdesc = smem_desc_sw128(smem_u32(vtiles), kGKeys * 128, 1024);
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            return __all_sync(0xffffffffu, mbar_wait(bar, parity, deadline)) != 0;
+        };
+        auto issue_pv = [&](int t) -> bool {
+            const int bb = t & 1, st = t % T::NSTV, pages = min(kGPages, npages - t * kGPages);
+            if (!wait(&full_v[st], (t / T::NSTV) & 1) || !wait(&p_full[bb], (t >> 1) & 1)) return false;
+            tc_fence_after();
+            const uint64_t vst = vdesc + (uint64_t)((st * T::TILE) >> 4);
+            const uint32_t pcol = tbase + T::COL_S + bb * kGKeys;
+#pragma unroll
+            for (int pg = 0; pg < kGPages; ++pg) {              // 16 keys each
+                if (pg >= pages) break;
+                const uint64_t vd = vst + (uint64_t)((pg * 2048) >> 4);
+                const uint32_t pc = pcol + 32 * (pg >> 1) + 8 * (pg & 1);
+                tc_mma_ts_if(on, tbase, pc, vd, T::IDESC_PV, (t > 0 || pg > 0) ? 1u : 0u);
+                if constexpr (T::PSPLIT) tc_mma_ts_if(on, tbase, pc + 16, vd, T::IDESC_PV, 1u);
+            }
+            tc_commit_if(on, &empty_v[st]);
+            tc_commit_if(on, &p_free[bb]);
+            return true;
+        };
+        bool ok = wait(q_full, 0);
+        for (int t = 0; t < nrounds && ok; ++t) {
+            const int bb = t & 1, st = t % T::NSTK;
+            // buffer bb holds P of round t - 2 until its products complete
+            ok = wait(&full_k[st], (t / T::NSTK) & 1) && (t < 2 || wait(&p_free[bb], ((t - 2) >> 1) & 1));
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t kst = kdesc + (uint64_t)((st * T::TILE) >> 4);
+            const uint32_t dcol = tbase + T::COL_S + bb * kGKeys;
+#pragma unroll
+            for (int kk = 0; kk < T::KSTEPS; ++kk)
+                tc_mma_ss_if(on, dcol, qdesc + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+                             kst + (uint64_t)(((kk >> 2) * (kGKeys * 128) + (kk & 3) * 32) >> 4), T::IDESC_S, kk > 0 ? 1u : 0u);
+            tc_commit_if(on, &empty_k[st]);
+            tc_commit_if(on, &s_full[bb]);
+            if (t >= 1) ok = issue_pv(t - 1);
+        }
+        if (ok) ok = issue_pv(nrounds - 1);
+        if (!ok && lane == 0) atomicOr(p.err, kDevErrTimeout);
+        // everything issued here, the arrivals above among it, completes before tensor
+        // memory is freed and the CTA leaves: in bounded time, so this wait has a
+        // deadline of its own (after a timeout the kernel's may have run out)
+        tc_commit_if(on, done);
+        if (!__all_sync(0xffffffffu, mbar_wait(done, 0, cycles() + kWaitDeadlineCycles)) && lane == 0)
+            atomicOr(p.err, kDevErrTimeout);
+    } else if constexpr (!T::FP4) {
+        // ---- producers: warp 5 streams the rounds' K tiles, warp 6 their V tiles.  The block
+        // ids come in windows of 32 pages, one per lane, the next window loaded when the
+        // current one starts.
+        const int kv = warp - 5;
+        const int ns = kv ? T::NSTV : T::NSTK;
+        uint64_t* fbar = kv ? full_v : full_k;
+        uint64_t* ebar = kv ? empty_v : empty_k;
+        uint8_t* tiles = kv ? vtiles : ktiles;
+        if (lane == 0) prefetch_tensormap(&tmap);
+        constexpr int IDW = 32 / kGPages;
+        uint32_t win = id_of(lane), nwin = id_of(32 + lane);
+        bool ok = true;
+        int issued = 0, nland = 0;
+        for (int t = 0; t < nrounds && !withhold; ++t) {
+            const int st = t % ns;
+            if (t > 0 && t % IDW == 0) {
+                win = nwin;
+                nwin = id_of((t / IDW + 1) * 32 + lane);
+            }
+            if (t >= ns && !__all_sync(0xffffffffu, mbar_wait(&ebar[st], ((t / ns) - 1) & 1, deadline))) {
+                ok = false;
+                break;
+            }
+            const int pg0 = t * kGPages, m = min(kGPages, npages - pg0);
+            // V rows that no query of the CTA sees (past the sequence's end, outside the
+            // window) may hold anything; the few page-heads with such rows are zeroed
+            // there before the round is handed on, so that P = 0 meets no NaN or Inf
+            bool dirty = false;
+            if (kv) {
+                for (int k = 0; k < m; ++k) {
+                    const int lp = page_of(pg0 + k);
+                    int z0 = 0, z1 = 0;
+                    if constexpr (WIN) span.hidden(lp, z0, z1);
+                    dirty |= z0 < z1 || total - lp * kBlockSize < kBlockSize;
+                }
+            }
+            uint64_t* fb = dirty ? landed : &fbar[st];
+            if (lane == 0) mbar_arrive_expect_tx(fb, (uint32_t)(m * T::CH * 2048));
+            __syncwarp();
+            // (one lane after another would cost each its own trip: one lane issues all)
+#pragma unroll
+            for (int pg = 0; pg < kGPages; ++pg) {
+                const uint32_t bj = __shfl_sync(0xffffffffu, win, (t % IDW) * kGPages + pg);
+                int prow = -32;                          // negative rows: TMA zero-fills
+                if (bj < p.num_blocks)
+                    prow = (int)(((p.layer * p.num_blocks + bj) * p.Hkv + (uint32_t)h) * 32u) + 16 * kv;
+                else if (kv == 0 && lane == 0 && pg < m)
+                    atomicOr(p.err, kDevErrBlockId);
+                if (pg < m && lane == 0)
+#pragma unroll
+                    for (int c = 0; c < T::CH; ++c)
+                        tma_load_2d(tiles + st * T::TILE + c * (kGKeys * 128) + pg * 2048, &tmap, fb, c * 64, prow);
+            }
+            if (dirty) {
+                // (its copies are waited for under a deadline of their own, below and here)
+                if (!__all_sync(0xffffffffu, mbar_wait(landed, nland & 1, cycles() + kWaitDeadlineCycles))) {
+                    ok = false;
+                    break;
+                }
+                ++nland;
+                for (int k = 0; k < m; ++k) {
+                    const int lp = page_of(pg0 + k);
+                    int z0 = 0, z1 = 0;
+                    if constexpr (WIN) span.hidden(lp, z0, z1);
+                    const int endr = total - lp * kBlockSize;
+                    for (int u = lane; u < kBlockSize * T::CH * 8; u += 32) {
+                        const int row = u & 15, cu = u >> 4;           // 16-B unit cu of the row
+                        if ((row >= z0 && row < z1) || row >= endr)
+                            *reinterpret_cast<uint4*>(tiles + st * T::TILE + (cu >> 3) * (kGKeys * 128) +
+                                                      (k * kBlockSize + row) * 128 + (cu & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&fbar[st]);
+            }
+            issued = t + 1;
+        }
+        if (lane == 0) {
+            if (!ok) atomicOr(p.err, kDevErrTimeout);
+            // drain: no TMA write may land after the CTA has exited.  The copies still in
+            // flight are this warp's last rounds in the ring; they land in bounded time, so the
+            // drain has a deadline of its own (the kernel's may have run out already)
+            const uint64_t drain_deadline = cycles() + kWaitDeadlineCycles;
+            for (int t = issued > ns ? issued - ns : 0; t < issued; ++t)
+                if (!mbar_wait(&fbar[t % ns], (t / ns) & 1, drain_deadline)) {
+                    atomicOr(p.err, kDevErrTimeout);
+                    break;
+                }
+        }
+    } else {
+        // ---- decoders: warp 5 the K halves, warp 6 the V halves of the records.  Each copies
+        // the halves that it reads into a ring of its own, refilling a slot once its codes
+        // are in registers; lanes resolve 32 pages at a time, one batch ahead.  A chunk is 16
+        // B, 32 codes of one row, with the scales of its two groups; codes times scales are
+        // exact in f16 and go to the tiles that TMA gives f16 pools: unit u of key row
+        // k at (u ^ (k % 8)) * 16 of its column.
+        using Rec = Fp4Rec<T::D>;
+        const int kv = warp - 5;
+        constexpr int U = T::D / 32, PER = U / 2;          // chunks of a row, of a lane and page-head
+        const int ns = kv ? T::NSTV : T::NSTK;
+        uint64_t* fbar = kv ? full_v : full_k;
+        uint64_t* ebar = kv ? empty_v : empty_k;
+        uint8_t* tiles = kv ? vtiles : ktiles;
+        uint8_t* ring = raw + kv * T::SLOTS * T::HALF;
+        uint64_t* rbar = full_r + kv * T::SLOTS;
+        auto resolve = [&](int o) {
+            const uint32_t blk = id_of(o);
+            if (blk < p.num_blocks) return (int)((p.layer * p.num_blocks + blk) * p.Hkv + (uint32_t)h);
+            if (o < npages) atomicOr(p.err, kDevErrBlockId);
+            return -1;
+        };
+        int issued = 0, taken = 0;
+        int cur = resolve(lane), nxt = resolve(32 + lane);
+        auto issue = [&]() {
+            if (issued >= npages || withhold) return;
+            const int rec = __shfl_sync(0xffffffffu, cur, issued & 31), s = issued % T::SLOTS;
+            uint8_t* slot = ring + s * T::HALF;
+            if (rec >= 0) {
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&rbar[s], T::HALF);
+                    bulk_load(slot, p.kv_data + (size_t)rec * Rec::BYTES + kv * T::HALF, T::HALF, &rbar[s]);
+                }
+            } else {
+                // a block id outside the pool (flagged): zeros, ordered before the slot's
+                // next asynchronous write
+                for (int k = lane; k < T::HALF / 16; k += 32) reinterpret_cast<uint4*>(slot)[k] = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&rbar[s]);
+            }
+            if ((++issued & 31) == 0) {
+                cur = nxt;
+                nxt = resolve(issued + 32 + lane);
+            }
+        };
+        for (int k = 0; k < T::SLOTS; ++k) issue();
+        bool ok = true;
+        for (int t = 0; t < nrounds && !withhold && ok; ++t) {
+            const int st = t % ns;
+            if (t >= ns && !__all_sync(0xffffffffu, mbar_wait(&ebar[st], ((t / ns) - 1) & 1, deadline))) {
+                ok = false;
+                break;
+            }
+            uint8_t* tile = tiles + st * T::TILE;
+            for (int pg = 0; pg < kGPages; ++pg) {
+                const int o = t * kGPages + pg;
+                uint4 w[PER];
+                uint32_t sc[PER];
+#pragma unroll
+                for (int i = 0; i < PER; ++i) { w[i] = make_uint4(0, 0, 0, 0); sc[i] = 0; }
+                if (o < npages) {
+                    const int s = o % T::SLOTS;
+                    if (!__all_sync(0xffffffffu, mbar_wait(&rbar[s], (o / T::SLOTS) & 1, deadline))) {
+                        ok = false;
+                        break;
+                    }
+                    taken = o + 1;
+                    const uint8_t* half = ring + s * T::HALF;
+                    const int pos0 = page_of(o) * kBlockSize;
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) {
+                        const int ch = lane + i * 32, u = ch % U, rr = ch / U, pos = pos0 + rr;
+                        // rows past the sequence's end, or that no query of the CTA sees: zeros
+                        if (pos < total && (!WIN || pos < span.sinks || pos >= span.lo)) {
+                            w[i] = *reinterpret_cast<const uint4*>(half + rr * Rec::CODE_ROW + u * 16);
+                            const uint8_t* scales = half + Rec::KS;
+                            sc[i] = kv == 0 ? *reinterpret_cast<const uint16_t*>(scales + rr * Rec::GROUPS + 2 * u)
+                                            : (uint32_t)scales[32 * u + rr] | ((uint32_t)scales[32 * u + 16 + rr] << 8);
+                        }
+                    }
+                    __syncwarp();
+                    issue();
+                }
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const int ch = lane + i * 32, u = ch % U, rr = ch / U, key = pg * 16 + rr;
+                    uint8_t* row = tile + (u >> 1) * (kGKeys * 128) + key * 128;
+                    const uint32_t s = e4m3x2_to_f16x2(sc[i]);
+                    const uint32_t s0 = __byte_perm(s, s, 0x1010u), s1 = __byte_perm(s, s, 0x3232u);
+                    const uint32_t word[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t f[4];
+                        fp4x8_to_f16(word[k], f);
+                        const uint32_t mm = k < 2 ? s0 : s1;
+                        *reinterpret_cast<uint4*>(row + ((((u & 1) * 4 + k) ^ (key & 7)) << 4)) =
+                            make_uint4(f16x2_mul(f[0], mm), f16x2_mul(f[1], mm), f16x2_mul(f[2], mm), f16x2_mul(f[3], mm));
+                    }
+                }
+            }
+            if (!ok) break;
+            // generic-proxy writes, read next by the tensor cores (async proxy)
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&fbar[st]);
+        }
+        if (!ok && lane == 0) atomicOr(p.err, kDevErrTimeout);
+        // drain: no copy may land after the CTA has exited; those not yet taken land in
+        // bounded time, under a deadline of their own
+        const uint64_t drain_deadline = cycles() + kWaitDeadlineCycles;
+        for (int o = taken; o < issued; ++o)
+            if (!mbar_wait(&rbar[o % T::SLOTS], (o / T::SLOTS) & 1, drain_deadline)) {
+                atomicOr(p.err, kDevErrTimeout);
+                break;
+            }
+    }
+    // tensor memory is freed by the warp that allocated it, after every use
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 4) {
+        tc_fence_after();
+        tmem_dealloc(tbase, 256);
+    }
+}
+
+template <class T, bool WIN>
+cudaError_t launch_grp(const PrefillLaunch& L) {
+    // the dynamic-smem opt-in is per device; remember it per device ordinal
+    static std::atomic<uint64_t> configured{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(configured.load() & bit)) {
+        cudaError_t e = cudaFuncSetAttribute(prefill_group_kernel<T, WIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+        if (e != cudaSuccess) return e;
+        configured.fetch_or(bit);
+    }
+    const PrefillParams& p = L.p;
+    // an upper bound on the CTAs: sum over b of ceil(n_b * group / 128) <= T * group / 128 + B
+    const uint64_t ctas = ((uint64_t)p.T * p.group + kGRows - 1) / kGRows + p.B;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas, p.Hkv);
+    cfg.blockDim = dim3(T::THREADS);
+    cfg.dynamicSmemBytes = T::SMEM;
+    cfg.stream = L.stream;
+    cudaLaunchAttribute attr[1];
+    if (p.flags & kDecodePdl) {
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    }
+    return cudaLaunchKernelEx(&cfg, prefill_group_kernel<T, WIN>, *L.tmap, p);
+}
+
+template <int D, int IO>
+cudaError_t launch_gd(const PrefillLaunch& L) {
+    if (L.kv_kind == kFP4)
+        return L.p.window > 0 ? launch_grp<Grp<D, IO, kFP4>, true>(L) : launch_grp<Grp<D, IO, kFP4>, false>(L);
+    return launch_grp<Grp<D, IO, IO>, true>(L);      // f16 / bf16 pools: windowed calls only
+}
+
+}  // namespace
+
+cudaError_t launch_group_prefill(const PrefillLaunch& L) {
+    if (L.head_dim == 64) return L.io_kind == kBF16 ? launch_gd<64, kBF16>(L) : launch_gd<64, kF16>(L);
+    return L.io_kind == kBF16 ? launch_gd<128, kBF16>(L) : launch_gd<128, kF16>(L);
+}
+
+}  // namespace vw
