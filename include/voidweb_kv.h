@@ -476,7 +476,7 @@ VW_API uint32_t vw_fault_pending(uint32_t kind);
  * clock cycles from the kernel's start (0 restores the default, about 2 s and
  * the normal launch), and they withhold copies -- the decode its query tiles,
  * the prefill its K/V tiles -- so that their first waits are ones that nothing
- * satisfies.  Such a launch records VW_DEV_ERR_TIMEOUT, waits (under the
+ * satisfies (the decode of a 4-bit pool has no such waits).  Such a launch records VW_DEV_ERR_TIMEOUT, waits (under the
  * default limit) for the copies and tensor-core operations it has in flight,
  * frees its tensor memory, and returns; its outputs are undefined (a prefill's
  * chunk append still runs).  vw_pool_check clears the word, after which the

@@ -328,8 +328,9 @@ def test_wait_that_runs_out_is_an_error_and_the_pool_recovers():
     out = torch.zeros_like(q)
     i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=bt.dev)  # noqa: E731
     bt.pool.set_wait_limit(20000)
-    bt.pool.paged_decode(0, q, table, lens, out)
-    assert bt.pool.check() & C.VW_DEV_ERR_TIMEOUT
+    bt.pool.paged_decode(0, q, table, lens, out)       # waits for nothing but its own loads
+    assert bt.pool.check() == 0
+    check(out, *decode_ref(bt, q), "bf16", "fp4")
     bt.pool.paged_prefill(0, q, i32(0, 1, 2), lens - 1, table, out)
     assert bt.pool.check() & C.VW_DEV_ERR_TIMEOUT
     bt.pool.set_wait_limit(0)

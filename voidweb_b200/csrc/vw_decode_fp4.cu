@@ -6,10 +6,12 @@
 //  * A page-head is 2304 B (head_dim 128), so at the memory's rate an SM has some 100
 //    cycles for each: what bounds this kernel is instructions and their
 //    latencies, not bytes.  The split of work among warps follows from that:
-//    every warp has a ring of its own, copies the pages that it will read (one
-//    bulk copy per page-head, issued by one lane as soon as the codes of an
-//    earlier page are in registers) and waits for nobody else's.  There are no
-//    producer warps, no empty barriers and no shared query ring.
+//    every warp has a ring of its own and copies the pages that it will read,
+//    16 B per lane (cp.async, whose groups complete in order), as soon as the codes
+//    of an earlier page are in registers.  There are no producer warps, no
+//    barriers while pages stream, and no shared query ring; nothing here waits for
+//    anything but its own copies.  (One bulk copy per page-head instead cost its
+//    warp some 300 cycles to issue.)
 //  * Warp w takes every W-th page-head of its CTA's range; the lanes resolve 32
 //    of its pages at a time, one batch ahead.
 //  * S^T = K Q^T and O^T = V^T P^T are m16n8k16 micro-tiles with the tokens as M (as K)
@@ -23,9 +25,6 @@
 //    2^-14: it adds some 1e-4 to the result's relative error, whose rounding to the
 //    io type is 2e-4 (f16) or 1.7e-3 (bf16) in the root mean square, and saves a
 //    quarter of the matrix instructions.
-//
-// Every wait is bounded; on timeout the kernel records kDevErrTimeout, waits for its
-// copies in flight and returns.
 #include <cuda_runtime.h>
 #include <atomic>
 #include <cstdint>
@@ -65,7 +64,7 @@ struct F4 {
     static constexpr int MERGE = W * 8 * (MROW + 2) * 4 + (W + 2) * 8 * 4;
     static constexpr int PFX = align_up_c((3 * kMaxBatchPerLaunch + 2) * 4, 128);
     static constexpr int RING = W * SW * Rec::BYTES;
-    static constexpr int SMEM = 128 + RING + align_up_c(MERGE, 128) + PFX + W * SW * 8 + 16;
+    static constexpr int SMEM = 128 + RING + align_up_c(MERGE, 128) + PFX;
     static_assert(SW >= PAIR && SW < 32, "a step's pages are in the ring together");
     static_assert(RING % 128 == 0 && SMEM <= 233472 / 2 - 1024, "two CTAs per SM");
 };
@@ -75,8 +74,6 @@ struct F4Smem {
     uint8_t* ring;      // [W][SW][BYTES]
     float *mo, *mm, *ml, *mf;   // one 8-head tile of the warp states, as in vw_decode.cu
     int *pfx, *nzp, *slen;
-    uint64_t* full;     // [W][SW]
-    int* flag;          // [0] abort
 };
 
 template <class T>
@@ -91,9 +88,6 @@ __device__ __forceinline__ F4Smem<T> f4_carve(uint8_t* p) {
     s.pfx = reinterpret_cast<int*>(p);
     s.nzp = s.pfx + (kMaxBatchPerLaunch + 1);
     s.slen = s.nzp + (kMaxBatchPerLaunch + 1);
-    p += T::PFX;
-    s.full = reinterpret_cast<uint64_t*>(p);
-    s.flag = reinterpret_cast<int*>(s.full + T::W * T::SW);
     return s;
 }
 
@@ -255,7 +249,6 @@ struct Feed {
     const DecodeParams& p;
     const F4Smem<T>& sm;
     uint8_t* ring;
-    uint64_t* full;
     int begin, n, warp, lane;
     int issued = 0;              // pages issued; those of batch issued/32 are in cur
     int cur, nxt;
@@ -277,28 +270,28 @@ struct Feed {
         return (int)((p.layer * p.num_blocks + blk) * p.Hkv + (uint32_t)h);
     }
 
-    // (the whole warp) copy the next page into its slot, which is free
+    // (the whole warp) copy the next page into its slot, which is free.  Every call ends a
+    // group, so that page k is in group k whether it exists or not.
     __device__ __forceinline__ void issue() {
-        if (warp + issued * T::W >= n || (p.flags & kDecodeWithholdQ)) return;
-        const int rec = __shfl_sync(0xffffffffu, cur, issued & 31);
-        const int s = issued % T::SW;
-        uint8_t* st = ring + s * T::Rec::BYTES;
-        if (rec >= 0) {
-            if (lane == 0) {
-                mbar_arrive_expect_tx(&full[s], T::Rec::BYTES);
-                bulk_load(st, p.kv_data + (size_t)rec * T::Rec::BYTES, T::Rec::BYTES, &full[s]);
+        if (warp + issued * T::W < n) {
+            const int rec = __shfl_sync(0xffffffffu, cur, issued & 31);
+            uint8_t* st = ring + issued % T::SW * T::Rec::BYTES;
+            const uint8_t* src = p.kv_data + (size_t)rec * T::Rec::BYTES;
+            if (rec >= 0) {
+#pragma unroll
+                for (int k = 0; k < T::Rec::BYTES / 16; k += 32)
+                    if (k + 32 <= T::Rec::BYTES / 16 || k + lane < T::Rec::BYTES / 16)
+                        cp_async16(st + (k + lane) * 16, src + (k + lane) * 16);
+            } else {
+                // a block id outside the pool (flagged): a record of zeros
+                for (int k = lane; k < T::Rec::BYTES / 16; k += 32) reinterpret_cast<uint4*>(st)[k] = make_uint4(0, 0, 0, 0);
             }
-        } else {
-            // a record of zeros, ordered before the slot's next asynchronous write
-            for (int k = lane; k < T::Rec::BYTES / 16; k += 32) reinterpret_cast<uint4*>(st)[k] = make_uint4(0, 0, 0, 0);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[s]);
+            if ((++issued & 31) == 0) {
+                cur = nxt;
+                nxt = resolve(issued + 32 + lane);
+            }
         }
-        if ((++issued & 31) == 0) {
-            cur = nxt;
-            nxt = resolve(issued + 32 + lane);
-        }
+        cp_async_commit();
     }
 };
 
@@ -454,12 +447,7 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
     extern __shared__ __align__(128) uint8_t smem_raw[];
     const F4Smem<T> sm = f4_carve<T>(smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
-    const uint64_t deadline = cycles() + (p.wait_cycles ? p.wait_cycles : kWaitDeadlineCycles);
     constexpr int W = T::W, NTH = T::THREADS;
-    uint64_t* full = sm.full + warp * T::SW;
-    if (lane < T::SW) mbar_init(&full[lane], 1);
-    fence_mbar_init();
-    if (tid == 0) sm.flag[0] = 0;
     // Programmatic dependent launch, as in vw_decode.cu: without early pages
     // everything waits for the predecessor; the combine may launch at once.
     const bool pdl = (p.flags & kDecodePdl) != 0, early = pdl && (p.flags & kDecodeEarlyPages) != 0;
@@ -488,7 +476,7 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
     }
     if (begin >= end) return;
 
-    Feed<T, WIN> feed{p, sm, sm.ring + warp * T::SW * T::Rec::BYTES, full, begin, end - begin, warp, lane};
+    Feed<T, WIN> feed{p, sm, sm.ring + warp * T::SW * T::Rec::BYTES, begin, end - begin, warp, lane};
     feed.cur = feed.resolve(lane);
     for (int k = 0; k < T::SW; ++k) feed.issue();
     feed.nxt = feed.resolve(32 + lane);
@@ -496,7 +484,6 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
 
     const int Hkv = (int)p.Hkv, g = (int)p.group;
     const bool append = p.k_new != nullptr;
-    bool alive = true;
     int done = 0;                         // the warp's pages consumed
     for (int x = begin; x < end;) {
         const int b = find_seq(sm.pfx, (int)p.B, Hkv, x);
@@ -534,34 +521,29 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
             }
             return true;
         };
-        // wait for the warp's page `done` + ahead
-        auto arrived = [&](int ahead) {
-            const int k = done + ahead;
-            if (__all_sync(0xffffffffu, mbar_wait(&full[k % T::SW], (k / T::SW) & 1, deadline))) return true;
-            if (lane == 0) set_err(p.err, kDevErrTimeout);
-            return false;
-        };
         auto slot = [&](int ahead) { return feed.ring + (done + ahead) % T::SW * T::Rec::BYTES; };
-        for (int i = warp + done * W; i < i_end && alive; i = warp + done * W) {
+        for (int i = warp + done * W; i < i_end; i = warp + done * W) {
             const int pg = pg0 + (i - i_base);
+            // SW + done groups are committed: the oldest one or two have to be there, for
+            // this lane, then (__syncwarp) for all
             if (whole(pg)) {
                 if (T::PAIR == 2 && i + W < i_end && whole(pg + W)) {
-                    alive = arrived(0) && arrived(1);
-                    if (!alive) break;
+                    cp_async_wait<T::SW - 2>();
+                    __syncwarp();
                     uint8_t* const st[2] = {slot(0), slot(1)};
                     step<T, WIN, 2, false>(p, feed, st, 0, qf, s, lane);
                     done += 2;
                 } else {
-                    alive = arrived(0);
-                    if (!alive) break;
+                    cp_async_wait<T::SW - 1>();
+                    __syncwarp();
                     uint8_t* const st[1] = {slot(0)};
                     step<T, WIN, 1, false>(p, feed, st, 0, qf, s, lane);
                     done += 1;
                 }
                 continue;
             }
-            alive = arrived(0);
-            if (!alive) break;
+            cp_async_wait<T::SW - 1>();
+            __syncwarp();
             uint8_t* const st[1] = {slot(0)};
             const int lp = WIN ? span.page(pg) : pg;
             uint32_t seen = 0xFFFFu;
@@ -596,8 +578,6 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
                     seen &= ~((0xFFFFu >> (16 - (z - a))) << a);
                 }
             }
-            // plain stores into a slot that a bulk copy fills next
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             step<T, WIN, 1, true>(p, feed, st, seen, qf, s, lane);
             done += 1;
@@ -605,13 +585,11 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
 
         // ---- merge the W warps' states for this segment, one 8-head tile at a time
         // (three barriers per tile), as in vw_decode.cu
-        if (!alive && lane == 0) sm.flag[0] = 1;     // abort marker, read by all warps below
         float* mo = sm.mo + warp * 8 * T::MROW;
         uint16_t* out = reinterpret_cast<uint16_t*>(p.out);
         const int piece = (x == begin) ? 0 : 1;
         float* po = p.part_o + ((size_t)blockIdx.x * 2 + piece) * T::G * T::D;
         float* pml = p.part_ml + ((size_t)blockIdx.x * 2 + piece) * T::G * 2;
-        bool abort = false;
 #pragma unroll
         for (int nt = 0; nt < T::NT; ++nt) {
 #pragma unroll
@@ -635,7 +613,6 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
                 sm.ml[warp * 8 + jl + 1] = s.l[nt][1];
             }
             __syncthreads();
-            abort = sm.flag[0] != 0;
             const int jn = min(8, g - nt * 8);    // live query heads of the tile
             if (tid < jn) {
                 float M = -INFINITY;
@@ -653,7 +630,7 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
                 sm.mf[(W + 1) * 8 + tid] = Ls;
             }
             __syncthreads();
-            for (int idx = tid; idx < jn * T::D && !abort; idx += NTH) {
+            for (int idx = tid; idx < jn * T::D; idx += NTH) {
                 const int jt = idx / T::D, d = idx - jt * T::D, j = nt * 8 + jt;
                 float Os = 0.0f;
 #pragma unroll
@@ -670,17 +647,8 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
             __syncthreads();
         }
         x += cnt;
-        if (abort) break;
     }
-    // never leave while a copy may still write this CTA's shared memory: after a timeout
-    // the warp's copies in flight (pages done .. issued - 1) land in bounded time,
-    // under a deadline of their own
-    const uint64_t drain_deadline = cycles() + kWaitDeadlineCycles;
-    for (int k = done; k < feed.issued; ++k)
-        if (!mbar_wait(&full[k % T::SW], (k / T::SW) & 1, drain_deadline)) {
-            set_err(p.err, kDevErrTimeout);
-            break;
-        }
+    // (each warp has consumed every page that it copied: none is in flight)
 }
 
 template <class T, bool WIN>

@@ -14,8 +14,7 @@
 //    per CTA, 4593.)
 //  * Warps 0-3: softmax, one row per thread.  Warp 4 issues the matrix instructions.
 //    f16 / bf16 pages: warp 5 streams K tiles, warp 6 V tiles (TMA).  4-bit pages:
-//    warp 5 copies the records' K halves into a ring and expands them into f16
-//    tiles, warp 6 the V halves.
+//    warp 5 expands the records' K halves into f16 tiles, warp 6 the V halves.
 //  * bf16 probabilities are a pair hi + lo (two P V products, as in vw_prefill.cu),
 //    those of f16 and 4-bit pages one f16.
 //  * Every wait is bounded; on timeout the kernel records kDevErrTimeout, waits
@@ -52,17 +51,14 @@ struct Grp {
     static constexpr int TILE = CH * kGKeys * 128;            // one K or V tile
     // K tiles and V tiles: a K tile frees when S of its round completes, rounds before the V
     // tile of that round, so where shared memory allows the K ring is one deeper
-    static constexpr int NSTK = D == 64 ? 4 : FP4 ? 2 : 3;
+    static constexpr int NSTK = D == 64 ? 4 : 3;
     static constexpr int NSTV = D == 64 ? 4 : 2;
-    // 4-bit record halves in the ring of the K decoder, and of the V decoder
-    static constexpr int HALF = FP4 ? Fp4Rec<D>::HALF : 0;
-    static constexpr int SLOTS = FP4 ? 7 * (128 / D) : 0;
     static constexpr int KSTEPS = D / 16;
     static constexpr int COL_S = D;                           // O in columns [0, D), two S buffers after it
-    // full, empty of K and V tiles; s_full, p_full, p_free of both buffers; q_full, landed, done; raw rings
-    static constexpr int NBAR = 2 * NSTK + 2 * NSTV + 9 + 2 * SLOTS;
+    // full, empty of K and V tiles; s_full, p_full, p_free of both buffers; q_full, landed, done
+    static constexpr int NBAR = 2 * NSTK + 2 * NSTV + 9;
     static constexpr int TPFX = pf_align((kMaxBatchPerLaunch + 1) * 4, 128);
-    static constexpr int SMEM = QTILE + (NSTK + NSTV) * TILE + 2 * SLOTS * HALF + NBAR * 8 + 16;
+    static constexpr int SMEM = QTILE + (NSTK + NSTV) * TILE + NBAR * 8 + 16;
     static constexpr int THREADS = 7 * 32;
     static constexpr uint32_t IDESC_S = idesc_f16(MBF, false, 128, kGKeys);
     static constexpr uint32_t IDESC_PV = idesc_f16(MBF, true, 128, D);
@@ -70,7 +66,6 @@ struct Grp {
     static_assert(2 * (SMEM + 1024) <= 233472, "two CTAs per SM");
     static_assert(3 * (SMEM + 1024) > 233472, "at most two CTAs per SM (tensor memory)");
     static_assert(TPFX <= TILE, "the tile prefix fits in a V tile");
-    static_assert(HALF % 16 == 0 && SLOTS < 32, "ring slots: 16-B aligned, issued within a batch of ids");
 };
 
 template <class T, bool WIN>
@@ -85,9 +80,8 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
     uint8_t* qs = smem_raw;
     uint8_t* ktiles = qs + T::QTILE;
     uint8_t* vtiles = ktiles + T::NSTK * T::TILE;
-    uint8_t* raw = vtiles + T::NSTV * T::TILE;          // 4-bit records
     int* tpfx = reinterpret_cast<int*>(vtiles + (T::NSTV - 1) * T::TILE);   // prologue only
-    uint64_t* full_k = reinterpret_cast<uint64_t*>(raw + 2 * T::SLOTS * T::HALF);
+    uint64_t* full_k = reinterpret_cast<uint64_t*>(vtiles + T::NSTV * T::TILE);
     uint64_t* empty_k = full_k + T::NSTK;
     uint64_t* full_v = empty_k + T::NSTK;
     uint64_t* empty_v = full_v + T::NSTV;
@@ -97,8 +91,7 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
     uint64_t* q_full = p_free + 2;
     uint64_t* landed = q_full + 1;
     uint64_t* done = landed + 1;
-    uint64_t* full_r = done + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full_r + 2 * T::SLOTS);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint64_t deadline = cycles() + (p.wait_cycles ? p.wait_cycles : kWaitDeadlineCycles);
     // test hook (vw_debug_set_wait_limit): no K/V tile is filled
@@ -112,7 +105,6 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
         mbar_init(q_full, 4);
         mbar_init(landed, 1);
         mbar_init(done, 1);
-        for (int s = 0; s < 2 * T::SLOTS; ++s) mbar_init(&full_r[s], 1);
         fence_mbar_init();
     }
     if (p.flags & kDecodePdl) griddep_wait();          // q, chunk rows and pages from the predecessor
@@ -497,96 +489,85 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
                 }
         }
     } else {
-        // ---- decoders: warp 5 the K halves, warp 6 the V halves of the records.  Each copies
-        // the halves that it reads into a ring of its own, refilling a slot once its codes
-        // are in registers; lanes resolve 32 pages at a time, one batch ahead.  A chunk is 16
+        // ---- decoders: warp 5 the K halves, warp 6 the V halves of the records.  A chunk is 16
         // B, 32 codes of one row, with the scales of its two groups; codes times scales are
         // exact in f16 and go to the tiles that TMA gives f16 pools: unit u of key row
-        // k at (u ^ (k % 8)) * 16 of its column.
+        // k at (u ^ (k % 8)) * 16 of its column.  The chunks of a whole round are in registers,
+        // loaded while the round before is expanded: once a page-head's are used, those
+        // of the same place in the next round are on their way (one bulk copy per half
+        // instead cost its warp some 300 cycles to issue).  Lanes resolve 32 pages at a
+        // time, one batch ahead.
         using Rec = Fp4Rec<T::D>;
-        const int kv = warp - 5;
         constexpr int U = T::D / 32, PER = U / 2;          // chunks of a row, of a lane and page-head
+        const int kv = warp - 5;
+        // the lane's chunk of its rows: the 8 lanes of a store phase take two units of four
+        // rows, whose eight slots of a 128-B line differ (a lane order of 4 units by 2 rows met
+        // each slot twice; the tensor cores' operand reads leave no bandwidth for that)
+        const int chunk_u = U == 4 ? (lane & 1) | (lane >> 2 & 2) : lane & 1;
+        const int chunk_row = U == 4 ? (lane >> 1 & 3) | (lane >> 2 & 4) : lane >> 1;
         const int ns = kv ? T::NSTV : T::NSTK;
         uint64_t* fbar = kv ? full_v : full_k;
         uint64_t* ebar = kv ? empty_v : empty_k;
         uint8_t* tiles = kv ? vtiles : ktiles;
-        uint8_t* ring = raw + kv * T::SLOTS * T::HALF;
-        uint64_t* rbar = full_r + kv * T::SLOTS;
+        const uint8_t* data = p.kv_data + kv * Rec::HALF;
         auto resolve = [&](int o) {
             const uint32_t blk = id_of(o);
             if (blk < p.num_blocks) return (int)((p.layer * p.num_blocks + blk) * p.Hkv + (uint32_t)h);
             if (o < npages) atomicOr(p.err, kDevErrBlockId);
             return -1;
         };
-        int issued = 0, taken = 0;
+        int next = 0;                                      // the page that fetch loads
         int cur = resolve(lane), nxt = resolve(32 + lane);
-        auto issue = [&]() {
-            if (issued >= npages || withhold) return;
-            const int rec = __shfl_sync(0xffffffffu, cur, issued & 31), s = issued % T::SLOTS;
-            uint8_t* slot = ring + s * T::HALF;
-            if (rec >= 0) {
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(&rbar[s], T::HALF);
-                    bulk_load(slot, p.kv_data + (size_t)rec * Rec::BYTES + kv * T::HALF, T::HALF, &rbar[s]);
+        uint4 w[kGPages][PER];
+        uint32_t sc[kGPages][PER][2];                      // K: both scales in the first, V: one each
+        uint32_t shown = 0;                                // bit e * PER + i: the chunk holds keys
+        auto fetch = [&](int e) {
+            const int rec = __shfl_sync(0xffffffffu, cur, next & 31);
+            // (a page without a record reads record 0; nothing of it is used)
+            const uint8_t* half = data + (size_t)max(rec, 0) * Rec::BYTES;
+            const int pos0 = page_of(next) * kBlockSize;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int u = chunk_u, rr = chunk_row + 8 * i, pos = pos0 + rr;
+                w[e][i] = __ldg(reinterpret_cast<const uint4*>(half + rr * Rec::CODE_ROW + u * 16));
+                const uint8_t* scales = half + Rec::KS;
+                if (kv == 0) {
+                    sc[e][i][0] = __ldg(reinterpret_cast<const uint16_t*>(scales + rr * Rec::GROUPS + 2 * u));
+                } else {
+                    sc[e][i][0] = __ldg(scales + 32 * u + rr);
+                    sc[e][i][1] = __ldg(scales + 32 * u + 16 + rr);
                 }
-            } else {
-                // a block id outside the pool (flagged): zeros, ordered before the slot's
-                // next asynchronous write
-                for (int k = lane; k < T::HALF / 16; k += 32) reinterpret_cast<uint4*>(slot)[k] = make_uint4(0, 0, 0, 0);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&rbar[s]);
+                // rows past the sequence's end, that no query of the CTA sees, or of a block id
+                // outside the pool (flagged) become zeros
+                const uint32_t bit = 1u << (e * PER + i);
+                const bool in = next < npages && rec >= 0 && pos < total && (!WIN || pos < span.sinks || pos >= span.lo);
+                shown = in ? shown | bit : shown & ~bit;
             }
-            if ((++issued & 31) == 0) {
+            if ((++next & 31) == 0) {
                 cur = nxt;
-                nxt = resolve(issued + 32 + lane);
+                nxt = resolve(next + 32 + lane);
             }
         };
-        for (int k = 0; k < T::SLOTS; ++k) issue();
+#pragma unroll
+        for (int e = 0; e < kGPages; ++e) fetch(e);
         bool ok = true;
-        for (int t = 0; t < nrounds && !withhold && ok; ++t) {
+        for (int t = 0; t < nrounds && !withhold; ++t) {
             const int st = t % ns;
             if (t >= ns && !__all_sync(0xffffffffu, mbar_wait(&ebar[st], ((t / ns) - 1) & 1, deadline))) {
                 ok = false;
                 break;
             }
             uint8_t* tile = tiles + st * T::TILE;
-            for (int pg = 0; pg < kGPages; ++pg) {
-                const int o = t * kGPages + pg;
-                uint4 w[PER];
-                uint32_t sc[PER];
 #pragma unroll
-                for (int i = 0; i < PER; ++i) { w[i] = make_uint4(0, 0, 0, 0); sc[i] = 0; }
-                if (o < npages) {
-                    const int s = o % T::SLOTS;
-                    if (!__all_sync(0xffffffffu, mbar_wait(&rbar[s], (o / T::SLOTS) & 1, deadline))) {
-                        ok = false;
-                        break;
-                    }
-                    taken = o + 1;
-                    const uint8_t* half = ring + s * T::HALF;
-                    const int pos0 = page_of(o) * kBlockSize;
-#pragma unroll
-                    for (int i = 0; i < PER; ++i) {
-                        const int ch = lane + i * 32, u = ch % U, rr = ch / U, pos = pos0 + rr;
-                        // rows past the sequence's end, or that no query of the CTA sees: zeros
-                        if (pos < total && (!WIN || pos < span.sinks || pos >= span.lo)) {
-                            w[i] = *reinterpret_cast<const uint4*>(half + rr * Rec::CODE_ROW + u * 16);
-                            const uint8_t* scales = half + Rec::KS;
-                            sc[i] = kv == 0 ? *reinterpret_cast<const uint16_t*>(scales + rr * Rec::GROUPS + 2 * u)
-                                            : (uint32_t)scales[32 * u + rr] | ((uint32_t)scales[32 * u + 16 + rr] << 8);
-                        }
-                    }
-                    __syncwarp();
-                    issue();
-                }
+            for (int e = 0; e < kGPages; ++e) {
 #pragma unroll
                 for (int i = 0; i < PER; ++i) {
-                    const int ch = lane + i * 32, u = ch % U, rr = ch / U, key = pg * 16 + rr;
+                    const int u = chunk_u, rr = chunk_row + 8 * i, key = e * 16 + rr;
                     uint8_t* row = tile + (u >> 1) * (kGKeys * 128) + key * 128;
-                    const uint32_t s = e4m3x2_to_f16x2(sc[i]);
+                    const uint32_t both = kv == 0 ? sc[e][i][0] : sc[e][i][0] | (sc[e][i][1] << 8);
+                    const uint32_t s = e4m3x2_to_f16x2((shown >> (e * PER + i)) & 1u ? both : 0u);
                     const uint32_t s0 = __byte_perm(s, s, 0x1010u), s1 = __byte_perm(s, s, 0x3232u);
-                    const uint32_t word[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                    const uint32_t word[4] = {w[e][i].x, w[e][i].y, w[e][i].z, w[e][i].w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         uint32_t f[4];
@@ -596,22 +577,14 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
                             make_uint4(f16x2_mul(f[0], mm), f16x2_mul(f[1], mm), f16x2_mul(f[2], mm), f16x2_mul(f[3], mm));
                     }
                 }
+                fetch(e);
             }
-            if (!ok) break;
             // generic-proxy writes, read next by the tensor cores (async proxy)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&fbar[st]);
         }
         if (!ok && lane == 0) atomicOr(p.err, kDevErrTimeout);
-        // drain: no copy may land after the CTA has exited; those not yet taken land in
-        // bounded time, under a deadline of their own
-        const uint64_t drain_deadline = cycles() + kWaitDeadlineCycles;
-        for (int o = taken; o < issued; ++o)
-            if (!mbar_wait(&rbar[o % T::SLOTS], (o / T::SLOTS) & 1, drain_deadline)) {
-                atomicOr(p.err, kDevErrTimeout);
-                break;
-            }
     }
     // tensor memory is freed by the warp that allocated it, after every use
     tc_fence_before();
