@@ -36,10 +36,10 @@
 #include "vw_split.cuh"
 
 #ifndef VW_FP4_WARPS
-#define VW_FP4_WARPS 6
+#define VW_FP4_WARPS 8
 #endif
 #ifndef VW_FP4_STAGES
-#define VW_FP4_STAGES 4
+#define VW_FP4_STAGES 3
 #endif
 #ifndef VW_FP4_PAIR
 #define VW_FP4_PAIR 2
@@ -53,8 +53,11 @@ template <int D_, int NT_, int IO_>
 struct F4 {
     static constexpr int D = D_, NT = NT_, IO = IO_;
     using Rec = Fp4Rec<D>;
-    static constexpr int W = VW_FP4_WARPS, THREADS = W * 32;
-    static constexpr int PAIR = NT == 1 ? VW_FP4_PAIR : 1;   // interior page-heads per step
+    // Eight warps (128 registers) with one query-head tile: 64 sequences of 16,384 tokens, 8 KV
+    // heads, 244 us against 257 with six; two tiles need the 168 registers of six
+    static constexpr int W = NT == 1 ? VW_FP4_WARPS : 6, THREADS = W * 32;
+    // interior page-heads per step (one: 257 us in the same case)
+    static constexpr int PAIR = NT == 1 ? VW_FP4_PAIR : 1;
     static constexpr int SW = VW_FP4_STAGES * (128 / D);     // ring slots of a warp
     static constexpr int G = 8 * NT;
     static constexpr int KT = D / 16, MT = D / 16;
@@ -250,8 +253,14 @@ struct Feed {
     const F4Smem<T>& sm;
     uint8_t* ring;
     int begin, n, warp, lane;
+    int left;                    // pages not issued yet
     int issued = 0;              // pages issued; those of batch issued/32 are in cur
     int cur, nxt;
+    uint32_t in = 0, out = 0;    // byte offsets of the slot to fill and of the oldest page (the ring is no power of two)
+
+    static __device__ __forceinline__ uint32_t after(uint32_t s) {
+        return s + T::Rec::BYTES == T::SW * T::Rec::BYTES ? 0u : s + T::Rec::BYTES;
+    }
 
     __device__ __forceinline__ int resolve(int k) const {
         const int i = warp + k * T::W;
@@ -273,21 +282,23 @@ struct Feed {
     // (the whole warp) copy the next page into its slot, which is free.  Every call ends a
     // group, so that page k is in group k whether it exists or not.
     __device__ __forceinline__ void issue() {
-        if (warp + issued * T::W < n) {
+        if (left > 0) {
+            --left;
             const int rec = __shfl_sync(0xffffffffu, cur, issued & 31);
-            uint8_t* st = ring + issued % T::SW * T::Rec::BYTES;
-            const uint8_t* src = p.kv_data + (size_t)rec * T::Rec::BYTES;
+            uint8_t* st = ring + in;
+            in = after(in);
             if (rec >= 0) {
+                const uint8_t* src = p.kv_data + (size_t)rec * T::Rec::BYTES + lane * 16;
+                uint8_t* dst = st + lane * 16;
 #pragma unroll
                 for (int k = 0; k < T::Rec::BYTES / 16; k += 32)
-                    if (k + 32 <= T::Rec::BYTES / 16 || k + lane < T::Rec::BYTES / 16)
-                        cp_async16(st + (k + lane) * 16, src + (k + lane) * 16);
+                    if (k + 32 <= T::Rec::BYTES / 16 || k + lane < T::Rec::BYTES / 16) cp_async16(dst + k * 16, src + k * 16);
             } else {
                 // a block id outside the pool (flagged): a record of zeros
                 for (int k = lane; k < T::Rec::BYTES / 16; k += 32) reinterpret_cast<uint4*>(st)[k] = make_uint4(0, 0, 0, 0);
             }
             if ((++issued & 31) == 0) {
-                cur = nxt;
+                cur = __shfl_sync(0xffffffffu, nxt, lane);
                 nxt = resolve(issued + 32 + lane);
             }
         }
@@ -476,15 +487,18 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
     }
     if (begin >= end) return;
 
-    Feed<T, WIN> feed{p, sm, sm.ring + warp * T::SW * T::Rec::BYTES, begin, end - begin, warp, lane};
-    feed.cur = feed.resolve(lane);
+    Feed<T, WIN> feed{p, sm, sm.ring + warp * T::SW * T::Rec::BYTES, begin, end - begin, warp, lane,
+                      (end - begin - warp + W - 1) / W};
+    // (through a shuffle: a value that is itself a load's result would be waited for, with the
+    // loads around it, wherever it is used)
+    feed.cur = __shfl_sync(0xffffffffu, feed.resolve(lane), lane);
     for (int k = 0; k < T::SW; ++k) feed.issue();
     feed.nxt = feed.resolve(32 + lane);
     if (early) griddep_wait();            // q, k_new, v_new may come from the predecessor
 
     const int Hkv = (int)p.Hkv, g = (int)p.group;
     const bool append = p.k_new != nullptr;
-    int done = 0;                         // the warp's pages consumed
+    int i = warp;                         // the warp's next page of the range
     for (int x = begin; x < end;) {
         const int b = find_seq(sm.pfx, (int)p.B, Hkv, x);
         const int np = sm.pfx[b + 1] - sm.pfx[b];
@@ -521,30 +535,34 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
             }
             return true;
         };
-        auto slot = [&](int ahead) { return feed.ring + (done + ahead) % T::SW * T::Rec::BYTES; };
-        for (int i = warp + done * W; i < i_end; i = warp + done * W) {
+        auto slot = [&]() {
+            uint8_t* st = feed.ring + feed.out;
+            feed.out = Feed<T, WIN>::after(feed.out);
+            return st;
+        };
+        while (i < i_end) {
             const int pg = pg0 + (i - i_base);
-            // SW + done groups are committed: the oldest one or two have to be there, for
-            // this lane, then (__syncwarp) for all
+            // SW groups follow the last page consumed: the oldest one or two have to be there,
+            // for this lane, then (__syncwarp) for all
             if (whole(pg)) {
                 if (T::PAIR == 2 && i + W < i_end && whole(pg + W)) {
                     cp_async_wait<T::SW - 2>();
                     __syncwarp();
-                    uint8_t* const st[2] = {slot(0), slot(1)};
+                    uint8_t* const st[2] = {slot(), slot()};
                     step<T, WIN, 2, false>(p, feed, st, 0, qf, s, lane);
-                    done += 2;
+                    i += 2 * W;
                 } else {
                     cp_async_wait<T::SW - 1>();
                     __syncwarp();
-                    uint8_t* const st[1] = {slot(0)};
+                    uint8_t* const st[1] = {slot()};
                     step<T, WIN, 1, false>(p, feed, st, 0, qf, s, lane);
-                    done += 1;
+                    i += W;
                 }
                 continue;
             }
             cp_async_wait<T::SW - 1>();
             __syncwarp();
-            uint8_t* const st[1] = {slot(0)};
+            uint8_t* const st[1] = {slot()};
             const int lp = WIN ? span.page(pg) : pg;
             uint32_t seen = 0xFFFFu;
             if (pg == np - 1) {
@@ -580,7 +598,7 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
             }
             __syncwarp();
             step<T, WIN, 1, true>(p, feed, st, seen, qf, s, lane);
-            done += 1;
+            i += W;
         }
 
         // ---- merge the W warps' states for this segment, one 8-head tile at a time

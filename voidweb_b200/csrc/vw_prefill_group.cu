@@ -517,7 +517,9 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
             return -1;
         };
         int next = 0;                                      // the page that fetch loads
-        int cur = resolve(lane), nxt = resolve(32 + lane);
+        // (through a shuffle: a value that is itself a load's result would be waited for, with
+        // the loads around it, wherever it is used)
+        int cur = __shfl_sync(0xffffffffu, resolve(lane), lane), nxt = resolve(32 + lane);
         uint4 w[kGPages][PER];
         uint32_t sc[kGPages][PER][2];                      // K: both scales in the first, V: one each
         uint32_t shown = 0;                                // bit e * PER + i: the chunk holds keys
@@ -544,7 +546,7 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
                 shown = in ? shown | bit : shown & ~bit;
             }
             if ((++next & 31) == 0) {
-                cur = nxt;
+                cur = __shfl_sync(0xffffffffu, nxt, lane);
                 nxt = resolve(next + 32 + lane);
             }
         };
