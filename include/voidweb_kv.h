@@ -300,7 +300,10 @@ VW_API int32_t vw_paged_prefill(vw_pool* pool, const vw_prefill_args* args, void
  * VW_PREFILL_CAUSAL.  The chunk's append writes every row as before.  Pages
  * that no query of a 128-token tile sees are not read.  V rows that no query of
  * a tile sees may hold anything; one that another query of its tile sees must
- * be finite, as in vw_paged_prefill. */
+ * be finite, as in vw_paged_prefill.  These calls, and every prefill of a
+ * 4-bit pool, may split long contexts over the pool's split-K scratch when there
+ * are few query tiles: of one pool, they and its decodes must not run at the
+ * same time on different streams. */
 VW_API int32_t vw_paged_prefill_window(vw_pool* pool, const vw_prefill_args* args, const vw_window* window,
                                        void* stream);
 

@@ -350,3 +350,33 @@ def test_refusals():
     with pytest.raises(ValueError):
         bt.pool.gather(0, table[0], table.shape[1] * 16 + 1)
     assert bt.pool.check() == 0
+
+
+@pytest.mark.parametrize("kv,io,D,Hq,Hkv,window,sinks", [
+    ("fp4", "bf16", 128, 28, 4, 0, 0), ("fp4", "f16", 64, 16, 1, 0, 0), ("fp4", "f16", 128, 8, 8, 3000, 7),
+    ("bf16", "bf16", 128, 28, 4, 4000, 4), ("f16", "f16", 64, 6, 2, 2000, 40), ("bf16", "bf16", 128, 3, 1, 100000, 0)])
+@pytest.mark.parametrize("chunks", [[(6000, 5)], [(3001, 1), (100, 40)], [(8000, 33), (0, 9), (15, 1), (2000, 130)]],
+                         ids=["1", "2", "4"])
+def test_few_queries_over_long_contexts(kv, io, D, Hq, Hkv, window, sinks, chunks):
+    """The keys of a tile split over several CTAs and merged; decodes around it on the same stream share the scratch."""
+    from tests.paged_cases import v_scales
+    totals = [a + n for a, n in chunks]
+    bt = Batch(len(chunks) + D, kv, io, D, Hq, Hkv, totals).fill()
+    q = [bt.rows(n, Hq) for _, n in chunks]
+    cu = torch.tensor([0] + [n for _, n in chunks]).cumsum(0).int().to(bt.dev)
+    start = torch.tensor([a for a, _ in chunks], dtype=torch.int32, device=bt.dev)
+    qd = torch.cat(q).to(bt.dev)
+    out, dec, table = torch.full_like(qd, 7.0), [], bt.device_table()
+    last = torch.stack([x[-1] for x in q]).to(bt.dev)
+    for _ in range(2):
+        d = torch.zeros_like(last)
+        bt.pool.paged_decode(0, last, table, bt.lens(), d, window=window, sinks=sinks)
+        bt.pool.paged_prefill(0, qd, cu, start, table, out, window=window, sinks=sinks)
+        dec.append(d)
+    assert bt.pool.check() == 0
+    assert torch.equal(dec[0], dec[1])
+    for b, (a, n) in enumerate(chunks):
+        ref = attend(q[b], held(bt.k[b], kv), held(bt.v[b], kv), torch.arange(a, a + n), window, sinks,
+                     v_scale=v_scales(bt.v[b], kv))
+        check(out[int(cu[b]):int(cu[b + 1])], *ref, io, kv, f"chunk {b}")
+        check(dec[0][b:b + 1], *(x[-1:] for x in ref), io, kv, f"decode {b}")

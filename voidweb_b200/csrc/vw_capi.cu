@@ -135,6 +135,9 @@ struct vw_pool {
     // split-K scratch: two sets, alternated per decode launch so that two
     // overlapping launches (programmatic dependent launch) never share one
     size_t scratch_o = 0, scratch_ml = 0;
+    // the whole of the scratch as partial tiles of 128 rows (grouped prefill)
+    uint32_t part_tiles = 0;
+    int sms = 0;
     uint64_t launches = 0;
     uint64_t wait_cycles = 0;           // vw_debug_set_wait_limit (0: the default bound)
     // decode plan (vw_decode_plan) and the batch it was made for
@@ -262,7 +265,8 @@ int32_t vw_pool_create(const vw_pool_config* cfg, vw_pool** out) {
     cudaError_t e;
     int sms = 0;
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device);
-    p->grid = (sms > 0 ? sms : 148) * decode_ctas_per_sm();
+    p->sms = sms > 0 ? sms : 148;
+    p->grid = p->sms * decode_ctas_per_sm();
     if (c.kv_data) {
         p->data = static_cast<uint8_t*>(c.kv_data);
     } else {
@@ -288,6 +292,8 @@ int32_t vw_pool_create(const vw_pool_config* cfg, vw_pool** out) {
     const size_t n_ml = decode_scratch_floats_ml(p->grid);
     p->scratch_o = n_o;
     p->scratch_ml = n_ml;
+    // two sets for the decode; the prefill's partial tiles may use all of it
+    p->part_tiles = (uint32_t)(2 * n_ml / (128 * 2));
     if ((e = dev_alloc(&p->part_o, 2 * n_o * 4)) != cudaSuccess ||
         (e = dev_alloc(&p->part_ml, 2 * n_ml * 4)) != cudaSuccess ||
         (e = dev_alloc(&p->plan, plan_ints(p->grid) * 4)) != cudaSuccess ||
@@ -624,6 +630,10 @@ static int32_t prefill_launch(vw_pool* pool, const vw_prefill_args* a, void* str
     p.window = win.window;
     p.sinks = win.sinks;
     p.wait_cycles = pool->wait_cycles;
+    p.part_o = pool->part_o;
+    p.part_ml = pool->part_ml;
+    p.part_tiles = pool->part_tiles;
+    L.sms = pool->sms;
     L.tmap = &pool->tmap_half;
     L.head_dim = g.head_dim;
     L.kv_kind = g.kv_kind;

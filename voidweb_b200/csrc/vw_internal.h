@@ -98,12 +98,16 @@ struct PrefillParams {
     // are ones that nothing completes and run out
     uint64_t wait_cycles;
     uint32_t window, sinks;     // window > 0: the mask of PageSpan (both at most kMaxWindow)
+    float* part_o;              // [part_tiles][128][D] split-K partial outputs (grouped kernel)
+    float* part_ml;             // [part_tiles][128][2] (running max, sum)
+    uint32_t part_tiles;
 };
 
 struct PrefillLaunch {
     PrefillParams p;
     const CUtensorMap* tmap;    // the pool's 16-row half-page-head map
     uint32_t head_dim, kv_kind, io_kind;
+    int sms;
     cudaStream_t stream;
 };
 

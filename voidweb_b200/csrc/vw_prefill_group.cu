@@ -17,11 +17,16 @@
 //    warp 5 expands the records' K halves into f16 tiles, warp 6 the V halves.
 //  * bf16 probabilities are a pair hi + lo (two P V products, as in vw_prefill.cu),
 //    those of f16 and 4-bit pages one f16.
+//  * Few tiles (a short question over a long document) leave most SMs idle while a CTA
+//    walks all its keys, some 1.1 us per round: the rounds of a tile are then split over
+//    up to kMaxSplit CTAs, which leave unnormalised outputs with their maxima and sums
+//    in f32, and a small grid merges them.
 //  * Every wait is bounded; on timeout the kernel records kDevErrTimeout, waits
 //    for its copies and matrix instructions in flight and returns.
 #define VW_MBAR_SUSPEND_HINT_NS 0
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <algorithm>
 #include <atomic>
 #include <cstdint>
 
@@ -38,6 +43,8 @@ namespace {
 constexpr int kGRows = 128;                       // query rows per CTA
 constexpr int kGKeys = 64;                        // keys per round
 constexpr int kGPages = kGKeys / kBlockSize;
+constexpr int kMaxSplit = 8;
+constexpr int kMinRounds = 2;                     // rounds of a split, at least
 constexpr float kGRescale = 8.0f;                 // log2 units: p <= 2^8 against a stale max
 
 template <int D_, int IO_, int KV_>
@@ -67,6 +74,75 @@ struct Grp {
     static_assert(3 * (SMEM + 1024) > 233472, "at most two CTAs per SM (tensor memory)");
     static_assert(TPFX <= TILE, "the tile prefix fits in a V tile");
 };
+
+// Rounds of a tile (or of a part of them) as its CTA and the merge compute them.
+struct Rounds {
+    int all, per, parts;        // rounds of the tile, of a part, parts
+};
+__device__ __forceinline__ Rounds split_rounds(int npages, int splits) {
+    Rounds r;
+    r.all = (npages + kGPages - 1) / kGPages;
+    r.per = max((r.all + splits - 1) / splits, kMinRounds);
+    r.parts = (r.all + r.per - 1) / r.per;
+    return r;
+}
+
+// Prefix of the tiles of every sequence over the batch, by one warp.
+__device__ __forceinline__ void tile_prefix(const int32_t* cu_q, int B, int T, int g, int* tpfx, int lane) {
+    int run = 0;
+    if (lane == 0) tpfx[0] = 0;
+    for (int b0 = 0; b0 < B; b0 += 32) {
+        const int b = b0 + lane;
+        int nt = 0;
+        if (b < B) {
+            const int n = __ldg(cu_q + b + 1) - __ldg(cu_q + b);
+            // (a chunk past q's T rows is refused later)
+            nt = n > 0 ? (int)(((long long)min(n, T) * g + kGRows - 1) / kGRows) : 0;
+        }
+        int incl = nt;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += v;
+        }
+        if (b < B) tpfx[b + 1] = run + incl;
+        run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+}
+
+// The tile of CTA column `col` (the last tiles, which visit the most keys of a causal chunk,
+// come first): its sequence, rows and keys.  False: none, or a chunk outside q's
+// T rows or past its block-table row (bad).
+struct TileGeom {
+    int b, row0, q_off, n, cs, total, rows, npages;
+    PageSpan span;
+    bool bad;
+};
+template <bool WIN>
+__device__ __forceinline__ bool tile_geom(const PrefillParams& p, const int* tpfx, int col, TileGeom& t) {
+    const int x = tpfx[p.B] - 1 - col, g = (int)p.group;
+    t.bad = false;
+    if (x < 0) return false;
+    t.b = pf_find(tpfx, (int)p.B, x);
+    t.row0 = (x - tpfx[t.b]) * kGRows;                 // first row in its (sequence, KV head)
+    t.q_off = __ldg(p.cu_q + t.b);
+    t.n = __ldg(p.cu_q + t.b + 1) - t.q_off;
+    t.cs = __ldg(p.ctx_start + t.b);
+    t.total = t.cs + t.n;
+    t.bad = t.q_off < 0 || t.n > (int)p.T || t.q_off + t.n > (int)p.T || t.cs < 0 ||
+            (long long)t.cs + t.n > (long long)p.bt_stride * kBlockSize;
+    if (t.bad) return false;
+    t.rows = t.n * g;
+    const int tok0 = t.row0 / g, tok1 = (min(t.row0 + kGRows, t.rows) - 1) / g;
+    const int kend = p.causal ? t.cs + tok1 + 1 : t.total;         // keys [0, kend)
+    t.npages = (kend + kBlockSize - 1) / kBlockSize;   // pages visited (ordinals, mapped by span.page)
+    t.span = PageSpan{};
+    if constexpr (WIN) {
+        t.span = page_span(t.npages, t.cs + tok0, p.window, p.sinks);
+        t.npages = t.span.n;
+    }
+    return true;
+}
 
 template <class T, bool WIN>
 __global__ void __launch_bounds__(T::THREADS, 2)
@@ -108,59 +184,31 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
         fence_mbar_init();
     }
     if (p.flags & kDecodePdl) griddep_wait();          // q, chunk rows and pages from the predecessor
+    // the merge of a split launch may come up now: it waits for this whole grid
+    if (gridDim.z > 1) griddep_launch_dependents();
     const int g = (int)p.group;
-    // CTAs per sequence and KV head, prefix over the batch (warp 0)
-    if (warp == 0) {
-        int run = 0;
-        if (lane == 0) tpfx[0] = 0;
-        for (int b0 = 0; b0 < (int)p.B; b0 += 32) {
-            const int b = b0 + lane;
-            int nt = 0;
-            if (b < (int)p.B) {
-                const int n = __ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b);
-                // (a chunk past q's T rows is refused below)
-                nt = n > 0 ? (int)(((long long)min(n, (int)p.T) * g + kGRows - 1) / kGRows) : 0;
-            }
-            int incl = nt;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, incl, off);
-                if (lane >= off) incl += v;
-            }
-            if (b < (int)p.B) tpfx[b + 1] = run + incl;
-            run += __shfl_sync(0xffffffffu, incl, 31);
-        }
-    }
+    if (warp == 0) tile_prefix(p.cu_q, (int)p.B, (int)p.T, g, tpfx, lane);
     __syncthreads();
-    // the last CTAs of a causal chunk visit the most keys: they start first
     // (more CTAs than the grid: chunk offsets that are not those of T rows)
     if (tpfx[p.B] > (int)gridDim.x && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(p.err, kDevErrSeqLen);
-    const int x = tpfx[p.B] - 1 - (int)blockIdx.x;
-    if (x < 0) return;
-    const int b = pf_find(tpfx, (int)p.B, x);
-    const int row0 = (x - tpfx[b]) * kGRows;           // first row of the CTA in its (sequence, KV head)
-    const int q_off = __ldg(p.cu_q + b);
-    const int n = __ldg(p.cu_q + b + 1) - q_off;
-    const int cs = __ldg(p.ctx_start + b);
-    const int total = cs + n;
-    // the offsets come from device memory: a chunk outside q's T rows or past
-    // its block-table row is flagged and skipped
-    if (q_off < 0 || q_off + n > (int)p.T || cs < 0 || total > (int)(p.bt_stride * kBlockSize)) {
-        if (threadIdx.x == 0) atomicOr(p.err, kDevErrSeqLen);
+    TileGeom geo;
+    if (!tile_geom<WIN>(p, tpfx, (int)blockIdx.x, geo)) {
+        // the offsets come from device memory: such a chunk is flagged and skipped
+        if (geo.bad && threadIdx.x == 0) atomicOr(p.err, kDevErrSeqLen);
         return;
     }
-    const int h = blockIdx.y, rows = n * g;
-    const int tok0 = row0 / g, tok1 = (min(row0 + kGRows, rows) - 1) / g;
-    const int kend = p.causal ? cs + tok1 + 1 : total; // keys [0, kend)
-    int npages = (kend + kBlockSize - 1) / kBlockSize; // pages visited (ordinals, mapped by span.page)
-    PageSpan span{};
-    if constexpr (WIN) {
-        span = page_span(npages, cs + tok0, p.window, p.sinks);
-        npages = span.n;
-    }
-    const int nrounds = (npages + kGPages - 1) / kGPages;
-    const uint32_t* bt = p.block_tables + (size_t)b * p.bt_stride;
-    auto page_of = [&](int o) { return WIN ? span.page(o) : o; };
+    const PageSpan span = geo.span;
+    const int row0 = geo.row0, q_off = geo.q_off, cs = geo.cs, total = geo.total, rows = geo.rows;
+    const int h = blockIdx.y;
+    // this CTA's part of the rounds: page ordinals from page0 on
+    const Rounds rounds = split_rounds(geo.npages, (int)gridDim.z);
+    const int round0 = (int)blockIdx.z * rounds.per;
+    if (round0 >= rounds.all) return;
+    const int nrounds = min(rounds.per, rounds.all - round0), page0 = round0 * kGPages;
+    const int npages = min(geo.npages - page0, nrounds * kGPages);
+    const bool partial = rounds.parts > 1;
+    const uint32_t* bt = p.block_tables + (size_t)geo.b * p.bt_stride;
+    auto page_of = [&](int o) { return WIN ? span.page(page0 + o) : page0 + o; };
     auto id_of = [&](int o) { return o < npages ? __ldg(bt + page_of(o)) : 0xFFFFFFFFu; };
 
     if (warp == 4) {
@@ -322,11 +370,21 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
                 tc_fence_after();
                 const float inv = l > 0.0f ? 1.0f / l : 0.0f;
                 uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + qrow * T::D * 2;
+                const size_t part = ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * gridDim.z + blockIdx.z;
+                float* po = p.part_o + (part * kGRows + r) * T::D;
+                if (partial) *reinterpret_cast<float2*>(p.part_ml + (part * kGRows + r) * 2) = make_float2(m_ref, l);
 #pragma unroll 1
                 for (int c0 = 0; c0 < T::D; c0 += 32) {
                     float o[32];
                     tmem_ld32f(ocol + c0, o);
                     tmem_wait_ld();
+                    if (partial) {
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            *reinterpret_cast<float4*>(po + c0 + 4 * u) =
+                                make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                        continue;
+                    }
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         uint32_t w[4];
@@ -597,6 +655,64 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
     }
 }
 
+// Merge of a split tile: weights 2^(max_i - max) over its parts, as the decode's combine.  CTA
+// (tile, KV head, 4 rows): a row per warp, D/32 elements per lane, every part's loads in
+// flight together.  The geometry is computed while the parts still run.
+constexpr int kMergeRows = 4;
+
+template <class T, bool WIN>
+__global__ void __launch_bounds__(128) prefill_merge_kernel(const PrefillParams p, int splits) {
+    __shared__ int tpfx[kMaxBatchPerLaunch + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = (int)p.group;
+    if (warp == 0) tile_prefix(p.cu_q, (int)p.B, (int)p.T, g, tpfx, lane);
+    __syncthreads();
+    TileGeom geo;
+    const bool has = tile_geom<WIN>(p, tpfx, (int)blockIdx.x, geo);
+    griddep_wait();
+    if (!has) return;
+    const Rounds rounds = split_rounds(geo.npages, splits);
+    if (rounds.parts == 1) return;                     // written by its CTA
+    constexpr int PER = T::D / 32;
+    const size_t part0 = ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * splits;
+    const int r = (int)blockIdx.z * kMergeRows + warp, row = geo.row0 + r;
+    if (row >= geo.rows) return;
+    float2 ml[kMaxSplit], v[kMaxSplit][PER / 2];
+    float M = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kMaxSplit; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.0f);
+        if (i >= rounds.parts) continue;
+        ml[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((part0 + i) * kGRows + r) * 2));
+        const float* po = p.part_o + ((part0 + i) * kGRows + r) * T::D + lane * PER;
+#pragma unroll
+        for (int e = 0; e < PER / 2; ++e) v[i][e] = __ldcg(reinterpret_cast<const float2*>(po) + e);
+    }
+#pragma unroll
+    for (int i = 0; i < kMaxSplit; ++i) M = fmaxf(M, ml[i].x);
+    float l = 0.0f, o[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMaxSplit; ++i) {
+        if (ml[i].x == -INFINITY) continue;            // no such part, or one without a key the row sees
+        const float w = ex2(ml[i].x - M);
+        l += w * ml[i].y;
+#pragma unroll
+        for (int e = 0; e < PER / 2; ++e) {
+            o[2 * e] += w * v[i][e].x;
+            o[2 * e + 1] += w * v[i][e].y;
+        }
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const int tq = row / g;
+    uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) +
+                   (((size_t)(geo.q_off + tq) * p.Hq + (size_t)blockIdx.y * g + (row - tq * g)) * T::D + lane * PER) * 2;
+#pragma unroll
+    for (int e = 0; e < PER; e += 2)
+        reinterpret_cast<uint32_t*>(dst)[e / 2] =
+            (uint32_t)pf_f32_to_io<T::IO>(o[e] * inv) | ((uint32_t)pf_f32_to_io<T::IO>(o[e + 1] * inv) << 16);
+}
+
 template <class T, bool WIN>
 cudaError_t launch_grp(const PrefillLaunch& L) {
     // the dynamic-smem opt-in is per device; remember it per device ordinal
@@ -612,19 +728,35 @@ cudaError_t launch_grp(const PrefillLaunch& L) {
     const PrefillParams& p = L.p;
     // an upper bound on the CTAs: sum over b of ceil(n_b * group / 128) <= T * group / 128 + B
     const uint64_t ctas = ((uint64_t)p.T * p.group + kGRows - 1) / kGRows + p.B;
+    // Parts of a tile: while there is an SM for each, the scratch holds them, and a block-table
+    // row holds kMinRounds rounds for each.  (Llama-3-8B heads, 32 tokens behind 8192:
+    // 130.6 us whole, 32.7 in eight parts.  Two CTAs on an SM slow one another, so
+    // with two parts of 112 tiles, 40 tokens behind 1500 of 7 sequences, 40.2 us against
+    // 33.8 whole.)
+    const uint64_t tiles = ctas * p.Hkv, row_rounds = (p.bt_stride + kGPages - 1) / kGPages;
+    uint64_t splits = std::min<uint64_t>(L.sms, p.part_tiles) / tiles;
+    splits = std::min<uint64_t>({splits, kMaxSplit, row_rounds / kMinRounds});
+    if (splits < 1) splits = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas, p.Hkv);
+    cfg.gridDim = dim3((unsigned)ctas, p.Hkv, (unsigned)splits);
     cfg.blockDim = dim3(T::THREADS);
     cfg.dynamicSmemBytes = T::SMEM;
     cfg.stream = L.stream;
     cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     if (p.flags & kDecodePdl) {
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
     }
-    return cudaLaunchKernelEx(&cfg, prefill_group_kernel<T, WIN>, *L.tmap, p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, prefill_group_kernel<T, WIN>, *L.tmap, p);
+    if (e != cudaSuccess || splits == 1) return e;
+    cfg.gridDim = dim3((unsigned)ctas, p.Hkv, kGRows / kMergeRows);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, prefill_merge_kernel<T, WIN>, p, (int)splits);
 }
 
 template <int D, int IO>

@@ -11,7 +11,6 @@ on torch's current stream.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -260,9 +259,12 @@ class KvPool:
             if block_table.dim() != 1 or block_table.shape[0] * 16 < seq_len:
                 raise ValueError(f"block_table: {tuple(block_table.shape)} for {seq_len} tokens")
             self._check(("block_table", block_table, block_table.shape, 4))
-            # (the rows belong to the stream that writes them)
-            with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
-                ok, ov = (torch.empty((s.num_kv_heads, seq_len, s.head_dim), dtype=dt, device=self.device) for _ in "kv")
+            shape = (s.num_kv_heads, seq_len, s.head_dim)
+            if stream is None:
+                ok, ov = block_table.new_empty(shape, dtype=dt), block_table.new_empty(shape, dtype=dt)
+            else:                               # the rows belong to the stream that writes them
+                with torch.cuda.stream(stream):
+                    ok, ov = block_table.new_empty(shape, dtype=dt), block_table.new_empty(shape, dtype=dt)
             C.check(C.lib().vw_kv_gather(self._h, layer, _ptr(block_table), seq_len, _ptr(ok), _ptr(ov), None, None,
                                          _stream(stream, self._index)))
             return ok, ov, None, None
