@@ -50,3 +50,49 @@ def test_reference_codec_is_the_nearest_code():
                 far = (abs(row[i].item()) / s - codes).abs()
                 options |= {c * s for c in codes[far == far.min()].tolist()}
             assert abs(got[r, i].item()) in options and got[r, i] * row[i] >= 0
+
+
+def _borders_code(v):
+    """E2M1 magnitude code of a quotient, to nearest, ties to even."""
+    return (v > .25) * 1 + (v >= .75) + (v > 1.25) + (v >= 1.75) + (v > 2.5) + (v >= 3.5) + (v > 5)
+
+
+@pytest.mark.parametrize("io", ["bf16", "f16"])
+def test_products_decide_codes_as_quotients_do(io):
+    """vw_fp4.cuh's arithmetic, restated in f32: every magnitude of the io type as a group's maximum, and every magnitude
+    under every scale with an inverse one ulp off either way, against the real quotients."""
+    import numpy as np
+    f = np.float32
+    bits = np.arange(0, 0x7F80 if io == "bf16" else 0x7C00, dtype=np.uint16)
+    x = (bits.astype(np.uint32) << 16).view(f) if io == "bf16" else bits.view(np.float16).astype(f)
+
+    def e4m3(v):
+        e = np.maximum(np.floor(np.log2(np.maximum(v, 1e-300))), -6)
+        step = 2.0 ** (e - 3)
+        return np.minimum(np.round(v / step) * step, 448.0)
+
+    t = np.minimum(x, f(1048576)) * f(1 / 6)
+    c = t * f(513)
+    want = e4m3(np.minimum(x.astype(np.float64) / 6, 448))
+    assert (e4m3((c - (c - t)).astype(np.float64)) == want).all()
+    xs = x[(x > 0) & (x < 1e6)]
+    for s in np.unique(want[want > 0]):
+        real = _borders_code(xs.astype(np.float64) / s)
+        inv = f(1 / s)
+        for r in (inv, np.nextafter(inv, f(0)), np.nextafter(inv, f(np.inf))):
+            q = (xs * r + f(1536)) - f(1536)
+            assert (_borders_code(q.astype(np.float64)) == real).all(), s
+
+
+def test_division_by_heads_as_a_product():
+    """vw_kv_ops.cu's HeadDiv over row counts below 2^31."""
+    import random
+    rng = random.Random(1)
+    for d in list(range(1, 130)) + [1000, 65535]:
+        s = 0
+        while (1 << s) < d:
+            s += 1
+        m = ((1 << (31 + s)) + d - 1) // d
+        assert m < 1 << 32
+        for w in list(range(300)) + [2 ** 31 - 1 - i for i in range(300)] + [rng.randrange(2 ** 31) for _ in range(300)]:
+            assert w * m >> (31 + s) == w // d

@@ -5,11 +5,10 @@
 // (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives; to nearest even, saturating); a
 // group whose scale rounds to 0 holds zeros.  A code stands for code * s: two
 // times four significant bits between 2^-10 and 2688, exact in f16 and in bf16,
-// so the attention multiplies codes by scales in f16 and rounds nothing.  The
-// scale's quotient is an IEEE f32 division: the borders between E4M3 codes are
-// products of few bits, so it falls on the side the real quotient falls on.  The
-// elements' quotients: fp4_quotient.  NaN elements encode as 6 (the
-// conversion's rule) and do not count in amax.
+// so the attention multiplies codes by scales in f16 and rounds nothing.  Neither
+// quotient needs a division to fall on the right side of a border between codes
+// (fp4_scale_code, fp4_quotient).  NaN elements encode as 6 (the conversion's
+// rule) and do not count in amax.
 //
 // One page-head (16 tokens of one KV head) is one record of 18 D bytes, which one
 // bulk copy moves, a K half and a V half:
@@ -35,11 +34,26 @@ struct Fp4Rec {
 };
 static_assert(Fp4Rec<128>::BYTES == 2304 && Fp4Rec<64>::BYTES == 1152, "18 D bytes");
 
-// E4M3 scale code of a group with the given largest magnitude.
+// E4M3 scale code of a group with the given largest magnitude: amax / 6 as a product,
+// within 2^-23 (relative), rounded to 15 bits (x - (x * 2^k - ..), the splitting of a
+// product by a constant of Dekker's), which decides the code as the real quotient
+// does: a border b between codes times 6 has at most 7 significant bits and amax at
+// most 11, so amax / 6 is either b, and rounds to it, or off it by at least 2^-11 b.
+// (Past 2^20 every group saturates.)
 __device__ __forceinline__ uint32_t fp4_scale_code(float amax) {
+    const float t = __fmul_rn(fminf(amax, 1048576.0f), 1.0f / 6.0f), c = __fmul_rn(t, 513.0f);
     uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.0f), "f"(__fdiv_rn(amax, 6.0f)));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.0f), "f"(__fsub_rn(c, __fsub_rn(c, t))));
     return r & 0xFFu;
+}
+
+// f16 pair of codes times scales -> bf16 pair, exact: five or fewer mantissa bits, magnitudes
+// 0 or normal.  The f16 bits shifted into bf16's fields are the value times 2^-112.
+__device__ __forceinline__ uint32_t fp4_f16x2_to_bf16x2(uint32_t h) {
+    uint32_t r;
+    const uint32_t small = ((h >> 3) & 0x0FFF0FFFu) | (h & 0x80008000u);
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(small), "r"(0x77807780u));   // 2^112
+    return r;
 }
 
 // Two E4M3 codes (low byte first) -> f16 pair.

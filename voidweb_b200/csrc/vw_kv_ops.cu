@@ -46,6 +46,21 @@ __device__ __forceinline__ uint64_t pool_row(const PoolGeom& g, uint32_t layer, 
 
 constexpr uint32_t kRowsPerWarp = 4;     // a warp's loads of 4 rows are in flight together
 
+// The same with the division by Hkv as a product: floor(w / d) = (w * m) >> (31 + s) for
+// w < 2^31, s = ceil(log2 d), m = ceil(2^(31 + s) / d) (Granlund and Montgomery).
+struct HeadDiv {
+    uint32_t d, m, s;
+};
+HeadDiv head_div(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    return HeadDiv{d, (uint32_t)(((1ull << (31 + s)) + d - 1) / d), s};
+}
+__device__ __forceinline__ RowIdx row_index(uint32_t w, const HeadDiv& h) {
+    const uint32_t q = (uint32_t)(((uint64_t)w * h.m) >> (31 + h.s));
+    return RowIdx{q >> 1, q & 1u, w - q * h.d};
+}
+
 // 4-bit record of (layer, block, head).
 template <int D>
 __device__ __forceinline__ uint64_t fp4_record(const PoolGeom& g, uint32_t layer, uint32_t blk, uint32_t h) {
@@ -62,7 +77,8 @@ template <int D>
 __global__ void __launch_bounds__(256) fp4_append_kernel(PoolGeom g, uint8_t* __restrict__ data, uint32_t layer,
                                                          const uint16_t* __restrict__ k_new,
                                                          const uint16_t* __restrict__ v_new,
-                                                         const int64_t* __restrict__ slots, uint32_t n, uint32_t* err) {
+                                                         const int64_t* __restrict__ slots, uint32_t n, HeadDiv hd,
+                                                         uint32_t* err) {
     using R = Fp4Rec<D>;
     constexpr int WORDS = D / 8, N = kFp4Rows * WORDS / 32;      // chunks of a row, of a lane
     const uint32_t lane = threadIdx.x & 31;
@@ -76,7 +92,7 @@ __global__ void __launch_bounds__(256) fp4_append_kernel(PoolGeom g, uint8_t* __
         code[j] = nullptr;
         const uint32_t unit = j * 32 + lane, w = w0 + unit / WORDS, word = unit % WORDS;
         if (w >= rows) continue;
-        const RowIdx x = row_index(w, g.num_kv_heads);
+        const RowIdx x = row_index(w, hd);
         const int64_t slot = __ldg(slots + x.i);
         if (slot < 0) continue;
         if (slot >= (int64_t)g.num_blocks * kBlockSize) {
@@ -233,7 +249,7 @@ template <int D>
 __global__ void __launch_bounds__(256) fp4_gather_kernel(PoolGeom g, const uint8_t* __restrict__ data, uint32_t layer,
                                                          const uint32_t* __restrict__ block_table, uint32_t seq_len,
                                                          uint16_t* __restrict__ out_k, uint16_t* __restrict__ out_v,
-                                                         uint32_t* err) {
+                                                         HeadDiv hd, uint32_t* err) {
     using R = Fp4Rec<D>;
     constexpr int WORDS = D / 8, N = kFp4Rows * WORDS / 32;      // words of a row, words of a lane
     const uint32_t lane = threadIdx.x & 31;
@@ -246,7 +262,7 @@ __global__ void __launch_bounds__(256) fp4_gather_kernel(PoolGeom g, const uint8
         dst[j] = nullptr;
         const uint32_t unit = j * 32 + lane, w = w0 + unit / WORDS, word = unit % WORDS;
         if (w >= rows) continue;
-        const RowIdx x = row_index(w, g.num_kv_heads);      // x.i = the position p
+        const RowIdx x = row_index(w, hd);      // x.i = the position p
         const uint32_t blk = __ldg(block_table + x.i / kBlockSize);
         if (blk >= g.num_blocks) {
             if (word == 0) atomicOr(err, kDevErrBlockId);
@@ -267,7 +283,7 @@ __global__ void __launch_bounds__(256) fp4_gather_kernel(PoolGeom g, const uint8
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             h[k] = f16x2_mul(h[k], s2);
-            if (g.io_kind == kBF16) h[k] = pack2<true>(f16_bits_to_f32(h[k] & 0xFFFFu), f16_bits_to_f32(h[k] >> 16));
+            if (g.io_kind == kBF16) h[k] = fp4_f16x2_to_bf16x2(h[k]);
         }
         *reinterpret_cast<uint4*>(dst[j]) = make_uint4(h[0], h[1], h[2], h[3]);
     }
@@ -326,9 +342,10 @@ cudaError_t launch_kv_append(const PoolGeom& g, uint8_t* data, float* scales, ui
     const unsigned grid = (unsigned)((rows + 8 * kRowsPerWarp - 1) / (8 * kRowsPerWarp));
     if (g.kv_kind == kFP4) {
         const unsigned grid = (unsigned)((rows + 8 * kFp4Rows - 1) / (8 * kFp4Rows));
+        const HeadDiv hd = head_div(g.num_kv_heads);
         const uint16_t *k = static_cast<const uint16_t*>(k_new), *v = static_cast<const uint16_t*>(v_new);
-        if (g.head_dim == 128) fp4_append_kernel<128><<<grid, 256, 0, s>>>(g, data, layer, k, v, slots, n, err);
-        else fp4_append_kernel<64><<<grid, 256, 0, s>>>(g, data, layer, k, v, slots, n, err);
+        if (g.head_dim == 128) fp4_append_kernel<128><<<grid, 256, 0, s>>>(g, data, layer, k, v, slots, n, hd, err);
+        else fp4_append_kernel<64><<<grid, 256, 0, s>>>(g, data, layer, k, v, slots, n, hd, err);
         return cudaGetLastError();
     }
     kv_append_kernel<<<grid, 256, 0, s>>>(g, data, scales, layer,
@@ -353,9 +370,10 @@ cudaError_t launch_kv_gather(const PoolGeom& g, const uint8_t* data, const float
     const unsigned grid = (unsigned)((rows + 8 * kRowsPerWarp - 1) / (8 * kRowsPerWarp));
     if (g.kv_kind == kFP4) {
         const unsigned grid = (unsigned)((rows + 8 * kFp4Rows - 1) / (8 * kFp4Rows));
+        const HeadDiv hd = head_div(g.num_kv_heads);
         uint16_t *k = static_cast<uint16_t*>(out_k), *v = static_cast<uint16_t*>(out_v);
-        if (g.head_dim == 128) fp4_gather_kernel<128><<<grid, 256, 0, s>>>(g, data, layer, block_table, seq_len, k, v, err);
-        else fp4_gather_kernel<64><<<grid, 256, 0, s>>>(g, data, layer, block_table, seq_len, k, v, err);
+        if (g.head_dim == 128) fp4_gather_kernel<128><<<grid, 256, 0, s>>>(g, data, layer, block_table, seq_len, k, v, hd, err);
+        else fp4_gather_kernel<64><<<grid, 256, 0, s>>>(g, data, layer, block_table, seq_len, k, v, hd, err);
         return cudaGetLastError();
     }
     kv_gather_kernel<<<grid, 256, 0, s>>>(g, data, scales, layer, block_table, seq_len,
