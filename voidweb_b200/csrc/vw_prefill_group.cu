@@ -129,10 +129,10 @@ __device__ __forceinline__ bool tile_geom(const PrefillParams& p, const int* tpf
     t.n = __ldg(p.cu_q + t.b + 1) - t.q_off;
     t.cs = __ldg(p.ctx_start + t.b);
     t.total = t.cs + t.n;
-    t.bad = t.q_off < 0 || t.n > (int)p.T || t.q_off + t.n > (int)p.T || t.cs < 0 ||
+    t.rows = (int)((unsigned)t.n * (unsigned)g);
+    t.bad = t.q_off < 0 || t.n > (int)p.T || t.q_off > (int)p.T - t.n || t.cs < 0 || t.row0 < 0 || t.row0 >= t.rows ||
             (long long)t.cs + t.n > (long long)p.bt_stride * kBlockSize;
     if (t.bad) return false;
-    t.rows = t.n * g;
     const int tok0 = t.row0 / g, tok1 = (min(t.row0 + kGRows, t.rows) - 1) / g;
     const int kend = p.causal ? t.cs + tok1 + 1 : t.total;         // keys [0, kend)
     t.npages = (kend + kBlockSize - 1) / kBlockSize;   // pages visited (ordinals, mapped by span.page)
@@ -495,19 +495,17 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
             uint64_t* fb = dirty ? landed : &fbar[st];
             if (lane == 0) mbar_arrive_expect_tx(fb, (uint32_t)(m * T::CH * 2048));
             __syncwarp();
-            // (one lane after another would cost each its own trip: one lane issues all)
-#pragma unroll
-            for (int pg = 0; pg < kGPages; ++pg) {
-                const uint32_t bj = __shfl_sync(0xffffffffu, win, (t % IDW) * kGPages + pg);
+            // one box per lane: lane l copies column l % CH of page-head l / CH (from one lane, one
+            // after another: 197 us against 191 in the Qwen2.5-7B case)
+            const int pg = lane / T::CH, c = lane % T::CH;
+            const uint32_t bj = __shfl_sync(0xffffffffu, win, (t % IDW) * kGPages + (pg < kGPages ? pg : 0));
+            if (pg < m) {
                 int prow = -32;                          // negative rows: TMA zero-fills
                 if (bj < p.num_blocks)
                     prow = (int)(((p.layer * p.num_blocks + bj) * p.Hkv + (uint32_t)h) * 32u) + 16 * kv;
-                else if (kv == 0 && lane == 0 && pg < m)
+                else if (kv == 0 && c == 0)
                     atomicOr(p.err, kDevErrBlockId);
-                if (pg < m && lane == 0)
-#pragma unroll
-                    for (int c = 0; c < T::CH; ++c)
-                        tma_load_2d(tiles + st * T::TILE + c * (kGKeys * 128) + pg * 2048, &tmap, fb, c * 64, prow);
+                tma_load_2d(tiles + st * T::TILE + c * (kGKeys * 128) + pg * 2048, &tmap, fb, c * 64, prow);
             }
             if (dirty) {
                 // (its copies are waited for under a deadline of their own, below and here)
