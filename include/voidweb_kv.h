@@ -107,8 +107,8 @@ VW_API int32_t vw_pool_check(vw_pool* pool, uint32_t* device_error);
 /* Reshape-and-cache (no reference kernel; paging rule of
  * flash_attention.bm:132-140).  k_new, v_new: [num_tokens][num_kv_heads][head_dim]
  * io dtype; slot_mapping: [num_tokens] int64, slot = block*16 + offset, a
- * negative slot skips the token.  FP8 and 4-bit pools quantise each row on the
- * way in. */
+ * negative slot skips the token.  The slots of one call must be distinct.  FP8
+ * and 4-bit pools quantise each row on the way in. */
 VW_API int32_t vw_kv_append(vw_pool* pool, uint32_t layer, const void* k_new, const void* v_new,
                      const int64_t* slot_mapping, uint32_t num_tokens, void* stream);
 

@@ -380,3 +380,105 @@ def test_few_queries_over_long_contexts(kv, io, D, Hq, Hkv, window, sinks, chunk
                      v_scale=v_scales(bt.v[b], kv))
         check(out[int(cu[b]):int(cu[b + 1])], *ref, io, kv, f"chunk {b}")
         check(dec[0][b:b + 1], *(x[-1:] for x in ref), io, kv, f"decode {b}")
+
+
+@pytest.mark.parametrize("kv,window", [("fp4", 0), ("fp4", 5), ("bf16", 5)])
+def test_largest_batch(kv, window):
+    """1024 sequences (the most that a launch takes), decode and prefill, lengths 1 to 40."""
+    totals = [1 + (7 * i) % 40 for i in range(1024)]
+    bt = Batch(15, kv, "bf16", 64, 6, 2, totals, max_batch=1024).fill()
+    q = bt.rows(1024, 6)
+    out = torch.zeros_like(q).to(bt.dev)
+    start, cu = bt.lens() - 1, torch.arange(1025, dtype=torch.int32, device=bt.dev)
+    for f in ("decode", "prefill"):
+        if f == "decode":
+            bt.pool.paged_decode(0, q.to(bt.dev), bt.device_table(), bt.lens(), out, window=window, sinks=2 if window else 0)
+        else:
+            out.zero_()
+            bt.pool.paged_prefill(0, q.to(bt.dev), cu, start, bt.device_table(), out, window=window, sinks=2 if window else 0)
+        assert bt.pool.check() == 0
+        for b in range(0, 1024, 37):
+            ref = attend(q[b:b + 1], held(bt.k[b], kv), held(bt.v[b], kv), torch.tensor([totals[b] - 1]), window, 2 if window else 0)
+            check(out[b:b + 1], *ref, "bf16", kv, f"{f} {b}")
+    with pytest.raises(Exception):
+        bt.pool.paged_decode(0, torch.zeros(1025, 6, 64, dtype=torch.bfloat16, device=bt.dev),
+                             torch.zeros(1025, 3, dtype=torch.int32, device=bt.dev),
+                             torch.ones(1025, dtype=torch.int32, device=bt.dev),
+                             torch.zeros(1025, 6, 64, dtype=torch.bfloat16, device=bt.dev), window=window, sinks=2 if window else 0)
+
+
+@pytest.mark.parametrize("kv,window", [("fp4", 0), ("f16", 70)])
+def test_prefill_with_more_query_heads_than_rows_of_a_tile(kv, window):
+    """71 and 200 query heads on one KV head: one token's rows span tiles."""
+    for Hq in (71, 200):
+        chunks = [(90, 3), (0, 5)]
+        bt = Batch(Hq, kv, "f16", 64, Hq, 1, [a + n for a, n in chunks]).fill()
+        q = [bt.rows(n, Hq) for _, n in chunks]
+        cu = torch.tensor([0, 3, 8], dtype=torch.int32, device=bt.dev)
+        start = torch.tensor([90, 0], dtype=torch.int32, device=bt.dev)
+        out = torch.zeros(8, Hq, 64, dtype=torch.float16, device=bt.dev)
+        bt.pool.paged_prefill(0, torch.cat(q).to(bt.dev), cu, start, bt.device_table(), out, window=window)
+        assert bt.pool.check() == 0
+        for b, (a, n) in enumerate(chunks):
+            ref = attend(q[b], held(bt.k[b], kv), held(bt.v[b], kv), torch.arange(a, a + n), window)
+            check(out[int(cu[b]):int(cu[b + 1])], *ref, "f16", kv, f"{Hq} {b}")
+
+
+@pytest.mark.parametrize("kv,window", [("fp4", 0), ("fp4", 20), ("bf16", 20), ("bf16", 0)])
+def test_lengths_and_chunks_outside_the_tables(kv, window):
+    """Flagged; nothing is written for them; the other sequences are right."""
+    from voidweb_b200 import _lib as C
+    bt = Batch(16, kv, "bf16", 128, 8, 2, [100, 50, 300], stride_extra=0).fill()
+    q, table = bt.rows(3, 8), bt.device_table()
+    qd = q.to(bt.dev)
+    refs = [attend(q[b:b + 1], held(bt.k[b], kv), held(bt.v[b], kv), torch.tensor([n - 1]), window) for b, n in enumerate(bt.totals)]
+    for bad in (0, -5, 320 + 1, 2 ** 31 - 1, 2 ** 31 - 17):
+        out = torch.full_like(qd, 7.0)
+        bt.pool.paged_decode(0, qd, table, bt.lens([100, bad, 300]), out, window=window)
+        assert bt.pool.check() & C.VW_DEV_ERR_SEQ_LEN
+        for b in (0, 2):
+            check(out[b:b + 1], *refs[b], "bf16", kv, f"len {bad}")
+        assert bad > 0 or (out[1] == 7.0).all()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=bt.dev)  # noqa: E731
+    for cu, start in ((i32(0, 1, 2, 9), i32(99, 49, 299)), (i32(0, 1, 2, 2 ** 31 - 1), i32(99, 49, 299)),
+                      (i32(0, 1, 2, 3), i32(99, 49, 2 ** 31 - 2)), (i32(0, 1, 2, 3), i32(99, 49, -1))):
+        out = torch.full_like(qd, 7.0)
+        bt.pool.paged_prefill(0, qd, cu, start, table, out, window=window)
+        assert bt.pool.check() & C.VW_DEV_ERR_SEQ_LEN
+        for b in (0, 1):
+            check(out[b:b + 1], *refs[b], "bf16", kv, f"chunk {b}")
+        assert (out[2] == 7.0).all()
+
+
+def test_forward_pass_over_a_4_bit_pool():
+    """The engine's symbol: a prompt and decode steps through voidweb_forward_pass."""
+    import ctypes
+    import numpy as np
+    from voidweb_b200 import _lib as C
+    L, Hq, Hkv, D, n = 2, 8, 2, 128, 60
+    bt = Batch(17, "fp4", "bf16", D, Hq, Hkv, [n], layers=L)
+    lib, q = C.lib(), bt.rows(n, Hq)
+    table = np.ascontiguousarray(bt.table[0, :4].numpy().astype(np.uint32))
+
+    def step(first, count, prefill):
+        hq = torch.stack([q[first:first + count]] * L).pin_memory()
+        hk, hv = (torch.stack([x[0][first:first + count]] * L).pin_memory() for x in (bt.k, bt.v))
+        ho = torch.zeros_like(hq).pin_memory()
+        C.check(lib.vw_forward_bind(bt.pool.handle, hq.data_ptr(), hk.data_ptr(), hv.data_ptr(), ho.data_ptr()))
+        toks = (ctypes.c_uint32 * count)()
+        d = C.SeqDescriptor(7, ctypes.addressof(toks), count, table.ctypes.data, len(table), 1 if prefill else 0)
+        a = C.ForwardArgs(ctypes.addressof(d), 1, Hq * D, Hq, Hkv, L, 100, D, 0.0, 0, None)
+        assert lib.voidweb_forward_pass(ctypes.byref(a)) == 0, lib.vw_last_error()
+        return ho
+
+    lib.vw_forward_set_seq_len(7, 0)
+    try:
+        outs = [step(0, 57, True)] + [step(p, 1, False) for p in range(57, n)]
+    finally:
+        lib.vw_forward_release(7)
+        lib.vw_forward_bind(None, None, None, None, None)
+    assert bt.pool.check() == 0
+    ref = attend(q, held(bt.k[0], "fp4"), held(bt.v[0], "fp4"), torch.arange(n))
+    for l in range(L):
+        check(torch.cat([o[l] for o in outs]), *ref, "bf16", "fp4", f"layer {l}")
+        same_as_held(bt, l)

@@ -93,7 +93,7 @@ __device__ __forceinline__ void warp_prefixes(const uint32_t* seq_lens, int B, i
         if (b < B) {
             const int sl = (int)__ldg(seq_lens + b);
             if (slen) slen[b] = sl;
-            np = (sl + 15) >> 4;
+            np = pages_of(sl);
             if (sl <= 0 || np > bt_stride) {
                 if (report) set_err(err, kDevErrSeqLen);
                 np = sl <= 0 ? 0 : bt_stride;
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kCombineThreads, kCombineMinBlocks) combine_ke
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     auto pages = [&](int i) {
         const int sl = (int)__ldcg(p.seq_lens + i);
-        const int np = (sl + 15) >> 4;
+        const int np = pages_of(sl);
         if (WIN && sl > 0) return decode_span(sl, (int)p.bt_stride, p.window, p.sinks).n;
         return sl <= 0 ? 0 : min(np, (int)p.bt_stride);
     };

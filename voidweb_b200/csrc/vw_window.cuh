@@ -13,6 +13,9 @@
 
 namespace vw {
 
+// Pages of seq_len tokens (seq_len + 15 may not fit 31 bits).
+__device__ __forceinline__ int pages_of(int seq_len) { return (seq_len >> 4) + ((seq_len & 15) != 0); }
+
 struct PageSpan {
     int n;          // pages visited
     int ns;         // sink pages: ordinals below ns are the logical pages themselves
@@ -42,8 +45,8 @@ __device__ __forceinline__ PageSpan page_span(int np, int first, uint32_t window
 // A decode's span: seq_len tokens, the query at the last one.  A seq_len beyond
 // the block-table row (flagged by the decode) counts as the row's last token.
 __device__ __forceinline__ PageSpan decode_span(int seq_len, int bt_stride, uint32_t window, uint32_t sinks) {
-    const int np = min((seq_len + kBlockSize - 1) / kBlockSize, bt_stride);
-    return page_span(np, min(seq_len, np * kBlockSize) - 1, window, sinks);
+    const int np = min(pages_of(seq_len), bt_stride);
+    return page_span(np, min(seq_len - 1, (np - 1) * kBlockSize + kBlockSize - 1), window, sinks);
 }
 
 }  // namespace vw
