@@ -3,7 +3,8 @@
 The product is libvoidweb_kv.so (C ABI: include/voidweb_kv.h): hand-written
 sm_100a CUDA kernels for KV append, GQA split-K paged decode (optionally fused
 with the append), copy-on-write / compaction block copies, the block-table
-gather and FP8 E4M3 KV pages; plus the C++ block manager and radix prefix tree.
+gather, FP8 E4M3 and 4-bit KV pages, chunked prefill, and sliding windows with sinks
+in decode and prefill; plus the C++ block manager and radix prefix tree.
 This package is its Python host mirror (ctypes); it has no fallback path.
 """
 from ._lib import build, lib, VoidwebError  # noqa: F401

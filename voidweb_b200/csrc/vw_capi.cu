@@ -308,7 +308,7 @@ int32_t vw_pool_create(const vw_pool_config* cfg, vw_pool** out) {
         delete p;
         return cuda_fail(e, "vw_pool_create: memset");
     }
-    // (4-bit records move as plain bulk copies, without a tensor map)
+    // (the kernels of 4-bit pools copy records without a tensor map)
     int32_t rc = c.kv_dtype == VW_FP4_E2M1 ? VW_OK : encode_pool_map(p);
     if (rc != VW_OK) {
         pool_free_all(p);

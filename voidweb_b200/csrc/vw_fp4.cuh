@@ -10,8 +10,8 @@
 // (fp4_scale_code, fp4_quotient).  NaN elements encode as 6 (the conversion's
 // rule) and do not count in amax.
 //
-// One page-head (16 tokens of one KV head) is one record of 18 D bytes, which one
-// bulk copy moves, a K half and a V half:
+// One page-head (16 tokens of one KV head) is one record of 18 D bytes, a K half
+// and a V half:
 //   K codes [16][D/2]      element 2i in the low half of byte i
 //   K scales [16][D/16]    a token's groups together
 //   V codes [16][D/2]
