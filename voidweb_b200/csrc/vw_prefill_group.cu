@@ -144,6 +144,11 @@ __device__ __forceinline__ bool tile_geom(const PrefillParams& p, const int* tpf
     return true;
 }
 
+__device__ __forceinline__ uint4 bf16_to_f16x8(uint4 v) {
+    auto two = [](uint32_t w) { return pack2<false>(bf16_bits_to_f32(w & 0xFFFFu), bf16_bits_to_f32(w >> 16)); };
+    return make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
+}
+
 template <class T, bool WIN>
 __global__ void __launch_bounds__(T::THREADS, 2)
 prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillParams p) {
@@ -225,25 +230,50 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
         const int r = threadIdx.x, row = row0 + r;
         const bool live = row < rows;
         const int tq = live ? row / g : 0;
-        const size_t qrow = (size_t)(q_off + tq) * p.Hq + (size_t)h * g + (live ? row - tq * g : 0);
         {
-            // the query row into the swizzled K-major tile: 16-B unit u goes to column
-            // u / 8, unit (u % 8) ^ (r % 8); rotated first with rope_theta > 0
-            const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q) + qrow * T::D * 2;
-            constexpr int U = T::D / 8, HALF = U / 2;
+            // The warp's query rows into the swizzled K-major tile: 16-B unit u goes to column
+            // u / 8, unit (u % 8) ^ (r % 8); rotated first with rope_theta > 0.  A lane takes
+            // units u and u + D/16 (the pairs of the rotation) of a row in 512/D rows, all its loads
+            // in flight together.  (A row per lane, unit after unit, took 8700 cycles of some
+            // 57,000 that a tile of 17 rounds takes, these 4500.)
+            constexpr int HALF = T::D / 16, STEP = 32 / HALF, N = 32 / STEP;
+            constexpr bool CONV = T::FP4 && T::IO == kBF16;            // 4-bit pages compute in f16
+            const int u = lane % HALF, u2 = u + HALF;
+            uint4 lo[N], hi[N];
 #pragma unroll
-            for (int u = 0; u < HALF; ++u) {
-                uint4 lo = make_uint4(0, 0, 0, 0), hi = make_uint4(0, 0, 0, 0);
-                if (live) {
-                    lo = __ldg(reinterpret_cast<const uint4*>(src + u * 16));
-                    hi = __ldg(reinterpret_cast<const uint4*>(src + (u + HALF) * 16));
+            for (int i = 0; i < N; ++i) {
+                const int rr = i * STEP + lane / HALF, qr = row0 + warp * 32 + rr;      // the row, in the warp and overall
+                const int tok = __shfl_sync(0xffffffffu, tq, rr);
+                lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
+                if (qr < rows) {
+                    const uint4* src = reinterpret_cast<const uint4*>(
+                        reinterpret_cast<const uint8_t*>(p.q) +
+                        ((size_t)(q_off + tok) * p.Hq + (size_t)h * g + (qr - tok * g)) * T::D * 2);
+                    lo[i] = __ldg(src + u);
+                    hi[i] = __ldg(src + u2);
                 }
-                uint32_t e[4] = {lo.x, lo.y, lo.z, lo.w}, f[4] = {hi.x, hi.y, hi.z, hi.w};
-                if (p.rope_theta > 0.0f && live) {
-                    // pairs (d, d + D/2): element of unit u with that of unit u + D/16
-                    const float pos = (float)(cs + tq);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int rr = warp * 32 + i * STEP + lane / HALF;
+                uint4 a = lo[i], b = hi[i];
+                if (CONV && p.rope_theta <= 0.0f) a = bf16_to_f16x8(a), b = bf16_to_f16x8(b);
+                *reinterpret_cast<uint4*>(qs + (u >> 3) * 16384 + rr * 128 + (((u & 7) ^ (rr & 7)) << 4)) = a;
+                *reinterpret_cast<uint4*>(qs + (u2 >> 3) * 16384 + rr * 128 + (((u2 & 7) ^ (rr & 7)) << 4)) = b;
+            }
+            if (p.rope_theta > 0.0f) {
+                // in place, by the lane that wrote the units: out of the way of calls without it
+#pragma unroll 1
+                for (int i = 0; i < N; ++i) {
+                    const int rr = warp * 32 + i * STEP + lane / HALF;
+                    const float pos = (float)(cs + __shfl_sync(0xffffffffu, tq, i * STEP + lane / HALF));
+                    uint4* pa = reinterpret_cast<uint4*>(qs + (u >> 3) * 16384 + rr * 128 + (((u & 7) ^ (rr & 7)) << 4));
+                    uint4* pb = reinterpret_cast<uint4*>(qs + (u2 >> 3) * 16384 + rr * 128 + (((u2 & 7) ^ (rr & 7)) << 4));
+                    uint4 a = *pa, b = *pb;
+                    uint32_t e[4] = {a.x, a.y, a.z, a.w}, f[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
+                        // pairs (d, d + D/2)
                         float ar = pf_io_to_f32<T::IO>(e[w] & 0xFFFFu), ai = pf_io_to_f32<T::IO>(f[w] & 0xFFFFu);
                         float br = pf_io_to_f32<T::IO>(e[w] >> 16), bi = pf_io_to_f32<T::IO>(f[w] >> 16);
                         const int d = u * 8 + 2 * w;
@@ -252,19 +282,10 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
                         e[w] = (uint32_t)pf_f32_to_io<T::IO>(ar) | ((uint32_t)pf_f32_to_io<T::IO>(br) << 16);
                         f[w] = (uint32_t)pf_f32_to_io<T::IO>(ai) | ((uint32_t)pf_f32_to_io<T::IO>(bi) << 16);
                     }
+                    a = make_uint4(e[0], e[1], e[2], e[3]), b = make_uint4(f[0], f[1], f[2], f[3]);
+                    if (CONV) a = bf16_to_f16x8(a), b = bf16_to_f16x8(b);
+                    *pa = a, *pb = b;
                 }
-                if constexpr (T::FP4 && T::IO == kBF16) {          // 4-bit pages compute in f16
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        e[w] = pack2<false>(bf16_bits_to_f32(e[w] & 0xFFFFu), bf16_bits_to_f32(e[w] >> 16));
-                        f[w] = pack2<false>(bf16_bits_to_f32(f[w] & 0xFFFFu), bf16_bits_to_f32(f[w] >> 16));
-                    }
-                }
-                const int u2 = u + HALF;
-                *reinterpret_cast<uint4*>(qs + (u >> 3) * 16384 + r * 128 + (((u & 7) ^ (r & 7)) << 4)) =
-                    make_uint4(e[0], e[1], e[2], e[3]);
-                *reinterpret_cast<uint4*>(qs + (u2 >> 3) * 16384 + r * 128 + (((u2 & 7) ^ (r & 7)) << 4)) =
-                    make_uint4(f[0], f[1], f[2], f[3]);
             }
             // generic-proxy writes, read next by the tensor cores (async proxy)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -369,6 +390,7 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
             if (ok && __all_sync(0xffffffffu, mbar_wait(done, 0, deadline))) {
                 tc_fence_after();
                 const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                const size_t qrow = (size_t)(q_off + tq) * p.Hq + (size_t)h * g + (live ? row - tq * g : 0);
                 uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + qrow * T::D * 2;
                 const size_t part = ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * gridDim.z + blockIdx.z;
                 float* po = p.part_o + (part * kGRows + r) * T::D;
