@@ -482,3 +482,21 @@ def test_forward_pass_over_a_4_bit_pool():
     for l in range(L):
         check(torch.cat([o[l] for o in outs]), *ref, "bf16", "fp4", f"layer {l}")
         same_as_held(bt, l)
+
+
+@pytest.mark.parametrize("kv,window,chunks", [("fp4", 0, [(300, 1216)]), ("fp4", 333, [(900, 1216)]),
+                                              ("bf16", 333, [(900, 700), (0, 500), (77, 24)]),
+                                              ("bf16", 40, [(900, 1290)])])
+def test_prefill_of_more_tiles_than_are_resident(kv, window, chunks):
+    """304 and more tiles of 128 rows over 8 KV heads, where the SMs hold 296 together."""
+    bt = Batch(18, kv, "bf16", 128, 32, 8, [a + n for a, n in chunks]).fill()
+    q = [bt.rows(n, 32) for _, n in chunks]
+    ns = [n for _, n in chunks]
+    cu = torch.tensor([sum(ns[:i]) for i in range(len(ns) + 1)], dtype=torch.int32, device=bt.dev)
+    start = torch.tensor([a for a, _ in chunks], dtype=torch.int32, device=bt.dev)
+    out = torch.zeros(sum(ns), 32, 128, dtype=torch.bfloat16, device=bt.dev)
+    bt.pool.paged_prefill(0, torch.cat(q).to(bt.dev), cu, start, bt.device_table(), out, window=window, sinks=3 if window else 0)
+    assert bt.pool.check() == 0
+    for b, (a, n) in enumerate(chunks):
+        ref = attend(q[b], held(bt.k[b], kv), held(bt.v[b], kv), torch.arange(a, a + n), window, 3 if window else 0)
+        check(out[int(cu[b]):int(cu[b + 1])], *ref, "bf16", kv, f"chunk {b}")

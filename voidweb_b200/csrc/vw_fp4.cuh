@@ -78,21 +78,21 @@ __device__ __forceinline__ float fp4_inverse(uint32_t scale_code) {
 // x / s to a multiple of 2^-13, which decides the code as the real quotient does: x * inverse is within 2^-21 of
 // x / s (relative).  A border b between codes (.25, .75, .. 5) times s has at most 7 significant bits and x at most
 // 11, so x / s is either b, and the sum rounds to b exactly (b is a multiple of .25), or off it by at least
-// 2^-11 b >= 2^-13, a whole step.  Two additions instead of a division.
-__device__ __forceinline__ float fp4_quotient(float x, float inverse) {
-    return __fsub_rn(__fadd_rn(__fmul_rn(x, inverse), 1536.0f), 1536.0f);
+// 2^-11 b >= 2^-13, a whole step.  Two additions instead of a division, for two elements at once.
+__device__ __forceinline__ float2 fp4_quotient(float x, float y, float inverse) {
+    const float2 q = fma2(make_float2(x, y), make_float2(inverse, inverse), make_float2(-0.0f, -0.0f));
+    return add2(add2(q, make_float2(1536.0f, 1536.0f)), make_float2(-1536.0f, -1536.0f));
 }
 
 // Four elements -> four E2M1 codes, the first in the low half of the low byte.
 __device__ __forceinline__ uint32_t fp4_encode4(const float* v, float inverse) {
-    const float a = fp4_quotient(v[0], inverse), b = fp4_quotient(v[1], inverse);
-    const float c = fp4_quotient(v[2], inverse), d = fp4_quotient(v[3], inverse);
+    const float2 a = fp4_quotient(v[0], v[1], inverse), b = fp4_quotient(v[2], v[3], inverse);
     uint16_t r;
     asm("{\n\t.reg .b8 lo, hi;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 lo, %2, %1;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 hi, %4, %3;\n\t"
         "mov.b16 %0, {lo, hi};\n\t}"
-        : "=h"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
+        : "=h"(r) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
 
