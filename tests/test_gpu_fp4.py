@@ -500,3 +500,28 @@ def test_prefill_of_more_tiles_than_are_resident(kv, window, chunks):
     for b, (a, n) in enumerate(chunks):
         ref = attend(q[b], held(bt.k[b], kv), held(bt.v[b], kv), torch.arange(a, a + n), window, 3 if window else 0)
         check(out[int(cu[b]):int(cu[b + 1])], *ref, "bf16", kv, f"chunk {b}")
+
+
+def test_other_types_are_refused():
+    """Rows of the other 16-bit type, 16-bit floats for ids; bit patterns of the right size pass."""
+    bt = Batch(19, "fp4", "bf16", 64, 4, 2, [20]).fill()
+    pool, table, lens = bt.pool, bt.device_table(), bt.lens()
+    q = bt.rows(1, 4).to(bt.dev)
+    out = torch.empty_like(q)
+    want = pool.paged_decode(0, q, table, lens, out).clone()
+    for bad in (dict(q=q.half()), dict(q=q.float()), dict(out=out.half()), dict(seq_lens=lens.float()),
+                dict(block_tables=table.float()), dict(seq_lens=lens.long())):
+        args = dict(dict(q=q, block_tables=table, seq_lens=lens, out=out), **bad)
+        with pytest.raises(ValueError):
+            pool.paged_decode(0, args["q"], args["block_tables"], args["seq_lens"], args["out"])
+        with pytest.raises(ValueError):
+            pool.paged_decode(0, args["q"], args["block_tables"], args["seq_lens"], args["out"], window=3)
+    k = bt.k[0][:1].to(bt.dev)
+    slots = torch.zeros(1, dtype=torch.int64, device=bt.dev)
+    for kk, vv, ss in ((k.half(), k, slots), (k, k.float(), slots), (k, k, slots.int()), (k, k, slots.double())):
+        with pytest.raises(ValueError):
+            pool.append(0, kk, vv, ss)
+    got = torch.empty_like(out)
+    pool.paged_decode(0, q.view(torch.int16), table.view(torch.uint32), lens, got.view(torch.int16))
+    assert torch.equal(got, want)
+    assert pool.check() == 0

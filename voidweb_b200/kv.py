@@ -84,6 +84,7 @@ class KvPool:
                            _ptr(data) if data is not None else None,
                            _ptr(scales) if scales is not None else None)
         self._index = dev.index or 0
+        self._io = torch.bfloat16 if spec.io_dtype == "bf16" else torch.float16
         h = ctypes.c_void_p()
         C.check(C.lib().vw_pool_create(ctypes.byref(cfg), ctypes.byref(h)))
         self._h = h
@@ -141,12 +142,13 @@ class KvPool:
         C.check(C.lib().vw_debug_set_wait_limit(self._h, cycles))
 
     def _check(self, *tensors) -> None:
-        """Refuse a tensor the kernels would read wrongly: (name, tensor, shape, element bytes) each."""
-        for name, t, shape, size in tensors:
+        """Refuse a tensor the kernels would read wrongly: (name, tensor, shape, type) each.
+        Integers of the type's size (bit patterns, unsigned ids) pass too."""
+        for name, t, shape, dtype in tensors:
             if t is None:
                 continue
-            if t.shape != shape or t.element_size() != size:
-                raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype}, expected {shape} of {size}-byte elements")
+            if t.shape != shape or (t.dtype != dtype and (t.is_floating_point() or t.element_size() != dtype.itemsize)):
+                raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype}, expected {tuple(shape)} {dtype}")
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
             if t.get_device() != self._index:
@@ -159,7 +161,8 @@ class KvPool:
         n = k_new.shape[0]
         if self.spec.kv_dtype == "fp4":
             row = (n, self.spec.num_kv_heads, self.spec.head_dim)
-            self._check(("k_new", k_new, row, 2), ("v_new", v_new, row, 2), ("slot_mapping", slot_mapping, (n,), 8))
+            self._check(("k_new", k_new, row, self._io), ("v_new", v_new, row, self._io),
+                        ("slot_mapping", slot_mapping, (n,), torch.int64))
         C.check(C.lib().vw_kv_append(self._h, layer, _ptr(k_new), _ptr(v_new),
                                      _ptr(slot_mapping), n, _stream(stream, self._index)))
 
@@ -183,9 +186,10 @@ class KvPool:
         if win is not None or self.spec.kv_dtype == "fp4":
             s = self.spec
             rows, new = (B, Hq, s.head_dim), (B, s.num_kv_heads, s.head_dim)
-            self._check(("q", q, rows, 2), ("out", out, rows, 2),
-                        ("block_tables", block_tables, (B, block_tables.shape[-1]), 4),
-                        ("seq_lens", seq_lens, (B,), 4), ("k_new", k_new, new, 2), ("v_new", v_new, new, 2))
+            self._check(("q", q, rows, self._io), ("out", out, rows, self._io),
+                        ("block_tables", block_tables, (B, block_tables.shape[-1]), torch.int32),
+                        ("seq_lens", seq_lens, (B,), torch.int32), ("k_new", k_new, new, self._io),
+                        ("v_new", v_new, new, self._io))
         if rope_theta > 0.0:
             flags |= C.VW_DECODE_ROPE
         a = C.DecodeArgs(layer, B, Hq, block_tables.shape[1], _ptr(q), _ptr(block_tables),
@@ -219,10 +223,10 @@ class KvPool:
         if win is not None or self.spec.kv_dtype == "fp4":
             s, B = self.spec, ctx_start.shape[0]
             rows, new = (T, Hq, s.head_dim), (T, s.num_kv_heads, s.head_dim)
-            self._check(("q", q, rows, 2), ("out", out, rows, 2), ("cu_seqlens", cu_seqlens, (B + 1,), 4),
-                        ("ctx_start", ctx_start, (B,), 4),
-                        ("block_tables", block_tables, (B, block_tables.shape[-1]), 4),
-                        ("k_new", k_new, new, 2), ("v_new", v_new, new, 2))
+            self._check(("q", q, rows, self._io), ("out", out, rows, self._io),
+                        ("cu_seqlens", cu_seqlens, (B + 1,), torch.int32), ("ctx_start", ctx_start, (B,), torch.int32),
+                        ("block_tables", block_tables, (B, block_tables.shape[-1]), torch.int32),
+                        ("k_new", k_new, new, self._io), ("v_new", v_new, new, self._io))
         if causal:
             flags |= C.VW_PREFILL_CAUSAL
         if rope_theta > 0.0:
@@ -255,10 +259,10 @@ class KvPool:
         s = self.spec
         dt = torch.uint8 if s.kv_dtype == "fp8" else torch.int16
         if s.kv_dtype == "fp4":
-            dt = torch.bfloat16 if s.io_dtype == "bf16" else torch.float16
+            dt = self._io
             if block_table.dim() != 1 or block_table.shape[0] * 16 < seq_len:
                 raise ValueError(f"block_table: {tuple(block_table.shape)} for {seq_len} tokens")
-            self._check(("block_table", block_table, block_table.shape, 4))
+            self._check(("block_table", block_table, block_table.shape, torch.int32))
             shape = (s.num_kv_heads, seq_len, s.head_dim)
             if stream is None:
                 ok, ov = block_table.new_empty(shape, dtype=dt), block_table.new_empty(shape, dtype=dt)
