@@ -168,7 +168,8 @@ VW_API int32_t vw_paged_decode(vw_pool* pool, const vw_decode_args* args, void* 
  * must be > 0; a window of the sequence's length or more sees everything.
  * Pages without a visible key are neither resolved nor read, so their
  * block-table entries may hold anything (e.g. ids of blocks given back).
- * Every row sees its own token, so no row is empty. */
+ * Every row sees its own token, so no row is empty.  Under a window, and over
+ * 4-bit pools, block_table_stride is at most 2^26 (2^30 tokens). */
 typedef struct {
     uint32_t window;
     uint32_t sinks;

@@ -525,3 +525,27 @@ def test_other_types_are_refused():
     pool.paged_decode(0, q.view(torch.int16), table.view(torch.uint32), lens, got.view(torch.int16))
     assert torch.equal(got, want)
     assert pool.check() == 0
+
+
+@pytest.mark.parametrize("kv", ["fp4", "bf16"])
+def test_block_table_rows_past_31_bits_are_refused(kv):
+    """2^26 blocks are 2^30 tokens; one more is refused before a launch, by every call that takes a window or a 4-bit pool."""
+    import ctypes
+    from voidweb_b200 import _lib as C
+    bt = Batch(20, kv, "bf16", 64, 4, 2, [20]).fill()
+    table, lens, q = bt.device_table(), bt.lens(), bt.rows(1, 4).to(bt.dev)
+    out, cu = torch.full_like(q, 7.0), torch.tensor([0, 1], dtype=torch.int32, device=bt.dev)
+    ptr, h, win = (lambda t: ctypes.c_void_p(t.data_ptr())), bt.pool.handle, C.Window(5, 1)
+    st = torch.cuda.current_stream().cuda_stream
+    big = (1 << 26) + 1
+    d = C.DecodeArgs(0, 1, 4, big, ptr(q), ptr(table), ptr(lens), ptr(out), None, None, 0.0, 0, 0.0, 0)
+    p = C.PrefillArgs(0, 1, 1, 4, big, C.VW_PREFILL_CAUSAL, ptr(q), None, None, ptr(cu), ptr(lens - 1), ptr(table), ptr(out), 0.0, 0.0)
+    bad = C.VW_ERR_INVALID_ARG
+    assert C.lib().vw_paged_decode_window(h, ctypes.byref(d), ctypes.byref(win), st) == bad
+    assert C.lib().vw_paged_prefill_window(h, ctypes.byref(p), ctypes.byref(win), st) == bad
+    if kv == "fp4":
+        assert C.lib().vw_paged_decode(h, ctypes.byref(d), st) == bad
+        assert C.lib().vw_paged_decode_static(h, ctypes.byref(d), st) == bad
+        assert C.lib().vw_paged_prefill(h, ctypes.byref(p), st) == bad
+    torch.cuda.synchronize()
+    assert bt.pool.check() == 0 and (out == 7.0).all()

@@ -434,6 +434,14 @@ static int32_t window_validate(const vw_window* w, const char* what) {
     return VW_OK;
 }
 
+// Windows and 4-bit pools keep positions in 31 bits with room to add to them: table rows end
+// at kMaxWindow tokens.
+static int32_t stride_validate(const vw_pool* pool, uint32_t stride, const vw_window* w, const char* what) {
+    if ((w || pool->geom.kv_kind == kFP4) && stride > kMaxWindow / kBlockSize)
+        return fail(VW_ERR_INVALID_ARG, "%s: block_table_stride %u > %u", what, stride, kMaxWindow / kBlockSize);
+    return VW_OK;
+}
+
 // Split-K scratch given to a decode launch in place of the pool's own.
 struct DecodeScratch {
     float* o;
@@ -474,6 +482,8 @@ uint32_t segment_cost(const PoolGeom& g) {
 
 static int32_t decode_launch(vw_pool* pool, const vw_decode_args* a, cudaStream_t s,
                              const DecodeScratch* fixed = nullptr, const vw_window* window = nullptr) {
+    const int32_t bad = stride_validate(pool, a->block_table_stride, window, "vw_paged_decode");
+    if (bad != VW_OK) return bad;
     const PoolGeom& g = pool->geom;
     DecodeLaunch L{};
     DecodeParams& p = L.p;
@@ -589,6 +599,8 @@ static int32_t prefill_validate(const vw_pool* pool, const vw_prefill_args* a) {
 }
 
 static int32_t prefill_launch(vw_pool* pool, const vw_prefill_args* a, void* stream, const vw_window* window) {
+    const int32_t bad = stride_validate(pool, a->block_table_stride, window, "vw_paged_prefill");
+    if (bad != VW_OK) return bad;
     if (a->num_seqs == 0 || a->num_tokens == 0) return VW_OK;
     DeviceScope ds(pool->cfg.device);
     const PoolGeom& g = pool->geom;
