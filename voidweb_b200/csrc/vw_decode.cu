@@ -1143,6 +1143,8 @@ decode_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p) {
         begin = range_start(sm.pfx, sm.nzp, (int)p.B, (int)p.Hkv, cost, (int)blockIdx.x * vper);
         end = range_start(sm.pfx, sm.nzp, (int)p.B, (int)p.Hkv, cost, ((int)blockIdx.x + 1) * vper);
     }
+    // (a batch of no pages: the grids behind this one still come after those before it)
+    griddep_wait_if(early && blockIdx.x == 0 && begin >= end);
     if (begin >= end) return;
 
     if (warp >= T::W) {

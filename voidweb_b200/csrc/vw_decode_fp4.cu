@@ -488,6 +488,8 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
         begin = range_start(sm.pfx, sm.nzp, (int)p.B, (int)p.Hkv, cost, (int)blockIdx.x * vper);
         end = range_start(sm.pfx, sm.nzp, (int)p.B, (int)p.Hkv, cost, ((int)blockIdx.x + 1) * vper);
     }
+    // (a batch of no pages: the grids behind this one still come after those before it)
+    griddep_wait_if(early && blockIdx.x == 0 && begin >= end);
     if (begin >= end) return;
 
     Feed<T, WIN> feed{p, sm, sm.ring + warp * T::SW * T::Rec::BYTES, begin, end - begin, warp, lane,

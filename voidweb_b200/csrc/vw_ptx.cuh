@@ -161,6 +161,11 @@ __device__ __forceinline__ void cp_async_wait() {
 __device__ __forceinline__ void griddep_wait() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
+// The same where `on`, as one predicated instruction (a branch in the decode's prologue
+// cost its FP8 instance 0.5 us of 86).
+__device__ __forceinline__ void griddep_wait_if(bool on) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %0, 0;\n\t@p griddepcontrol.wait;\n\t}" ::"r"((uint32_t)on) : "memory");
+}
 // Let the next programmatic dependent grid start launching.
 __device__ __forceinline__ void griddep_launch_dependents() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -231,14 +231,24 @@ __global__ void __launch_bounds__(kCombineThreads, kCombineMinBlocks) combine_ke
         before += red[w][0]; all += red[w][1]; nz_before += red[w][2]; nz_all += red[w][3];
     }
     const int np = pages(b);
-    if (np == 0) return;
+    // A grid that launches on this one waits for it alone, so this one must not complete
+    // before the decode: its first CTA always waits (the others may return early, and
+    // make room for those with something to merge).
+    const bool first = blockIdx.x == 0 && blockIdx.y == 0;
+    if (np == 0) {
+        griddep_wait_if(first);
+        return;
+    }
     const int cost = (int)p.seg_cost;
     const int vper = virtual_per_cta(virtual_total(Hkv * all, Hkv * nz_all, cost), dec_grid);
     const int s_begin = Hkv * before + h * np;
     const int k = Hkv * nz_before + h;        // segment ordinal
     const int v0 = s_begin + cost * k;
     const int c0 = v0 / vper, c1 = (v0 + np - 1) / vper;
-    if (c0 == c1) return;                      // written out by the decode CTA itself
+    if (c0 == c1) {                            // written out by the decode CTA itself
+        griddep_wait_if(first);
+        return;
+    }
     // CTA c0 holds this segment in slot 0 when the segment starts its range
     // (the page before it, of segment k-1, lies in an earlier CTA), else in
     // slot 1 (its last segment); every later CTA starts inside it
