@@ -1143,8 +1143,10 @@ decode_kernel(const __grid_constant__ CUtensorMap tmap, const DecodeParams p) {
         begin = range_start(sm.pfx, sm.nzp, (int)p.B, (int)p.Hkv, cost, (int)blockIdx.x * vper);
         end = range_start(sm.pfx, sm.nzp, (int)p.B, (int)p.Hkv, cost, ((int)blockIdx.x + 1) * vper);
     }
-    // (a batch of no pages: the grids behind this one still come after those before it)
-    griddep_wait_if(early && blockIdx.x == 0 && begin >= end);
+    // (A batch of no pages: the grids behind this one still come after those before it.  The
+    // condition as one: nested in the return's branch it cost 64 FP8 sequences 0.9 us of 85,
+    // predicated 0.4, so 0.1.)
+    if (begin >= end && early && blockIdx.x == 0) griddep_wait();
     if (begin >= end) return;
 
     if (warp >= T::W) {

@@ -13,8 +13,9 @@
 
 namespace vw {
 
-// Pages of seq_len tokens (seq_len + 15 may not fit 31 bits).
-__device__ __forceinline__ int pages_of(int seq_len) { return (seq_len >> 4) + ((seq_len & 15) != 0); }
+// Pages of seq_len tokens; unsigned, since seq_len + 15 may not fit 31 bits.  (Callers
+// discard the result for lengths below 1.)
+__device__ __forceinline__ int pages_of(int seq_len) { return (int)(((uint32_t)seq_len + 15u) >> 4); }
 
 struct PageSpan {
     int n;          // pages visited
