@@ -123,6 +123,40 @@ __device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b) {
     return r;
 }
 
+// bf16 queries meet 4-bit pages in f16.  A row whose largest magnitude lies in [2^-1, 2^16) goes
+// as it is: its elements are multiples of 2^-24 or rounded to one, off by at most 2^-24 of
+// the largest.  Any other row (its large elements would be infinite, its small ones lost) is
+// multiplied by the power of two that brings its largest element to [2^14, 2^15), and the
+// row's scores by the inverse.  `top`: the row's largest magnitude, bf16 bits; a row of zeros
+// and one with an infinity or a NaN stay (1).
+constexpr uint32_t kQueryLow = 0x3F00u, kQueryHigh = 0x4780u;      // 2^-1, 2^16
+
+__device__ __forceinline__ float fp4_query_factor(uint32_t top) {
+    if (top == 0u || top >= 0x7F80u || (top >= kQueryLow && top < kQueryHigh)) return 1.0f;
+    return __uint_as_float((uint32_t)min(14 + 127 - (int)(top >> 7) + 127, 253) << 23);
+}
+__device__ __forceinline__ float fp4_query_unfactor(float factor) {      // 1 / factor, exactly
+    return __uint_as_float((254u << 23) - __float_as_uint(factor));
+}
+
+// bf16 pair times a power of two -> f16 pair.
+__device__ __forceinline__ uint32_t fp4_query_pair(uint32_t w, float factor) {
+    return pack2<false>(bf16_bits_to_f32(w & 0xFFFFu) * factor, bf16_bits_to_f32(w >> 16) * factor);
+}
+
+// The largest magnitude of N bf16 pairs (bits; NaN if one is).
+template <int N>
+__device__ __forceinline__ uint32_t bf16_top(const uint32_t (&w)[N]) {
+    uint32_t t[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) asm("abs.bf16x2 %0, %1;" : "=r"(t[k]) : "r"(w[k]));
+#pragma unroll
+    for (int n = N / 2; n > 0; n /= 2)
+#pragma unroll
+        for (int k = 0; k < n; ++k) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(t[k]) : "r"(t[k]), "r"(t[k + n]));
+    return max(t[0] & 0xFFFFu, t[0] >> 16);
+}
+
 // One row of a record by one warp: lane l holds elements l*D/32 .. +D/32-1 (the
 // first D/32 of v).  Writes codes and scales of token t into the records at rec
 // and, when rec2 is given, the same at rec2.

@@ -148,9 +148,22 @@ __device__ __forceinline__ bool tile_geom(const PrefillParams& p, const int* tpf
     return true;
 }
 
+// One lane's units a, b of a bf16 query row -> f16, times the row's factor; HALF neighbouring
+// lanes hold the row and get the factor.
+template <int HALF>
+__device__ __forceinline__ float query_to_f16(uint4& a, uint4& b) {
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, top = bf16_top<8>(w);
+#pragma unroll
+    for (int off = 1; off < HALF; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+    const float f = fp4_query_factor(top);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = fp4_query_pair(w[k], f);
+    a = make_uint4(w[0], w[1], w[2], w[3]), b = make_uint4(w[4], w[5], w[6], w[7]);
+    return f;
+}
+
 __device__ __forceinline__ uint4 bf16_to_f16x8(uint4 v) {
-    auto two = [](uint32_t w) { return pack2<false>(bf16_bits_to_f32(w & 0xFFFFu), bf16_bits_to_f32(w >> 16)); };
-    return make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
+    return make_uint4(fp4_query_pair(v.x, 1.0f), fp4_query_pair(v.y, 1.0f), fp4_query_pair(v.z, 1.0f), fp4_query_pair(v.w, 1.0f));
 }
 
 template <class T, bool WIN>
@@ -234,6 +247,7 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
         const int r = threadIdx.x, row = row0 + r;
         const bool live = row < rows;
         const int tq = live ? row / g : 0;
+        float scale_log2 = p.scale_log2;               // of this thread's row
         {
             // The warp's query rows into the swizzled K-major tile: 16-B unit u goes to column
             // u / 8, unit (u % 8) ^ (r % 8); rotated first with rope_theta > 0.  A lane takes
@@ -242,6 +256,7 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
             // 57,000 that a tile of 17 rounds takes, these 4500.)
             constexpr int HALF = T::D / 16, STEP = 32 / HALF, N = 32 / STEP;
             constexpr bool CONV = T::FP4 && T::IO == kBF16;            // 4-bit pages compute in f16
+            constexpr uint32_t FIRST = HALF == 8 ? 0x01010101u : 0x11111111u;      // the first lane of each row
             const int u = lane % HALF, u2 = u + HALF;
             uint4 lo[N], hi[N];
 #pragma unroll
@@ -257,15 +272,30 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
                     hi[i] = __ldg(src + u2);
                 }
             }
+            bool again = p.rope_theta > 0.0f;          // rows to rotate, or bf16 rows outside f16's range
+            if constexpr (CONV) {
+                bool high = false, low = false;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const uint32_t w[8] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w, hi[i].x, hi[i].y, hi[i].z, hi[i].w};
+                    const uint32_t own = bf16_top<8>(w);
+                    high |= own >= kQueryHigh;
+                    uint32_t big = __ballot_sync(0xffffffffu, own >= kQueryLow || row0 + warp * 32 + i * STEP + lane / HALF >= rows);
+#pragma unroll
+                    for (int off = 1; off < HALF; off <<= 1) big |= big >> off;
+                    low |= (big & FIRST) != FIRST;
+                }
+                again |= low || __any_sync(0xffffffffu, high);
+            }
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int rr = warp * 32 + i * STEP + lane / HALF;
                 uint4 a = lo[i], b = hi[i];
-                if (CONV && p.rope_theta <= 0.0f) a = bf16_to_f16x8(a), b = bf16_to_f16x8(b);
+                if (CONV && !again) a = bf16_to_f16x8(a), b = bf16_to_f16x8(b);
                 *reinterpret_cast<uint4*>(qs + (u >> 3) * 16384 + rr * 128 + (((u & 7) ^ (rr & 7)) << 4)) = a;
                 *reinterpret_cast<uint4*>(qs + (u2 >> 3) * 16384 + rr * 128 + (((u2 & 7) ^ (rr & 7)) << 4)) = b;
             }
-            if (p.rope_theta > 0.0f) {
+            if (again) {
                 // in place, by the lane that wrote the units: out of the way of calls without it
 #pragma unroll 1
                 for (int i = 0; i < N; ++i) {
@@ -276,7 +306,7 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
                     uint4 a = *pa, b = *pb;
                     uint32_t e[4] = {a.x, a.y, a.z, a.w}, f[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
+                    for (int w = 0; w < 4 && p.rope_theta > 0.0f; ++w) {
                         // pairs (d, d + D/2)
                         float ar = pf_io_to_f32<T::IO>(e[w] & 0xFFFFu), ai = pf_io_to_f32<T::IO>(f[w] & 0xFFFFu);
                         float br = pf_io_to_f32<T::IO>(e[w] >> 16), bi = pf_io_to_f32<T::IO>(f[w] >> 16);
@@ -287,7 +317,10 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
                         f[w] = (uint32_t)pf_f32_to_io<T::IO>(ai) | ((uint32_t)pf_f32_to_io<T::IO>(bi) << 16);
                     }
                     a = make_uint4(e[0], e[1], e[2], e[3]), b = make_uint4(f[0], f[1], f[2], f[3]);
-                    if (CONV) a = bf16_to_f16x8(a), b = bf16_to_f16x8(b);
+                    if (CONV) {
+                        const float f = __shfl_sync(0xffffffffu, query_to_f16<HALF>(a, b), lane % STEP * HALF);
+                        if (lane / STEP == i) scale_log2 *= fp4_query_unfactor(f);
+                    }
                     *pa = a, *pb = b;
                 }
             }
@@ -333,7 +366,7 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
                 for (int k = 0; k < kGKeys; k += 8)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) m4[c] = fmax3(m4[c], xs[k + 2 * c], xs[k + 2 * c + 1]);
-                const float tmax = fmaxf(fmax3(m4[0], m4[1], m4[2]), m4[3]) * p.scale_log2;
+                const float tmax = fmaxf(fmax3(m4[0], m4[1], m4[2]), m4[3]) * scale_log2;
                 const bool need = tmax > m_ref + kGRescale;
                 float alpha = 1.0f;
                 if (need) {
@@ -360,7 +393,7 @@ prefill_group_kernel(const __grid_constant__ CUtensorMap tmap, const PrefillPara
                 }
                 l *= alpha;
                 const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
-                const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), mu2 = make_float2(-mu, -mu);
+                const float2 sc2 = make_float2(scale_log2, scale_log2), mu2 = make_float2(-mu, -mu);
                 float2 ls[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                 // P over S: 32 keys take 16 columns of hi (or of the one f16) and, with a pair,
                 // 16 of lo
