@@ -302,9 +302,9 @@ VW_API int32_t vw_paged_prefill(vw_pool* pool, const vw_prefill_args* args, void
  * that no query of a 128-token tile sees are not read.  V rows that no query of
  * a tile sees may hold anything; one that another query of its tile sees must
  * be finite, as in vw_paged_prefill.  These calls, and every prefill of a
- * 4-bit pool, may split long contexts over the pool's split-K scratch when there
- * are few query tiles: of one pool, they and its decodes must not run at the
- * same time on different streams. */
+ * 4-bit pool, may split long contexts over scratch that the pool keeps for its
+ * prefills when there are few query tiles: two of them of one pool must not run at
+ * the same time on different streams (a decode may run beside either). */
 VW_API int32_t vw_paged_prefill_window(vw_pool* pool, const vw_prefill_args* args, const vw_window* window,
                                        void* stream);
 

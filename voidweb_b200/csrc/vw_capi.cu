@@ -135,8 +135,10 @@ struct vw_pool {
     // split-K scratch: two sets, alternated per decode launch so that two
     // overlapping launches (programmatic dependent launch) never share one
     size_t scratch_o = 0, scratch_ml = 0;
-    // the whole of the scratch as partial tiles of 128 rows (grouped prefill)
-    uint32_t part_tiles = 0;
+    // the grouped prefill's split tiles, at most one per SM: scratch of their own, so that a
+    // prefill may run beside a decode
+    float* tile_o = nullptr;            // [sms][128][head_dim]
+    float* tile_ml = nullptr;           // [sms][128][2]
     int sms = 0;
     uint64_t launches = 0;
     uint64_t wait_cycles = 0;           // vw_debug_set_wait_limit (0: the default bound)
@@ -167,6 +169,8 @@ void pool_free_all(vw_pool* p) {
     if (p->own_scales && p->scales) cudaFree(p->scales);
     if (p->part_o) cudaFree(p->part_o);
     if (p->part_ml) cudaFree(p->part_ml);
+    if (p->tile_o) cudaFree(p->tile_o);
+    if (p->tile_ml) cudaFree(p->tile_ml);
     if (p->plan) cudaFree(p->plan);
     if (p->err) cudaFree(p->err);
     if (p->stage) cudaFree(p->stage);
@@ -292,10 +296,11 @@ int32_t vw_pool_create(const vw_pool_config* cfg, vw_pool** out) {
     const size_t n_ml = decode_scratch_floats_ml(p->grid);
     p->scratch_o = n_o;
     p->scratch_ml = n_ml;
-    // two sets for the decode; the prefill's partial tiles may use all of it
-    p->part_tiles = (uint32_t)(2 * n_ml / (128 * 2));
+    const size_t tile_rows = (size_t)p->sms * kPrefillTileRows;
     if ((e = dev_alloc(&p->part_o, 2 * n_o * 4)) != cudaSuccess ||
         (e = dev_alloc(&p->part_ml, 2 * n_ml * 4)) != cudaSuccess ||
+        (e = dev_alloc(&p->tile_o, tile_rows * c.head_dim * 4)) != cudaSuccess ||
+        (e = dev_alloc(&p->tile_ml, tile_rows * 2 * 4)) != cudaSuccess ||
         (e = dev_alloc(&p->plan, plan_ints(p->grid) * 4)) != cudaSuccess ||
         (e = dev_alloc(&p->err, 4)) != cudaSuccess) {
         pool_free_all(p);
@@ -642,9 +647,8 @@ static int32_t prefill_launch(vw_pool* pool, const vw_prefill_args* a, void* str
     p.window = win.window;
     p.sinks = win.sinks;
     p.wait_cycles = pool->wait_cycles;
-    p.part_o = pool->part_o;
-    p.part_ml = pool->part_ml;
-    p.part_tiles = pool->part_tiles;
+    p.part_o = pool->tile_o;
+    p.part_ml = pool->tile_ml;
     L.sms = pool->sms;
     L.tmap = &pool->tmap_half;
     L.head_dim = g.head_dim;

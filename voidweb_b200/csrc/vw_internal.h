@@ -12,6 +12,7 @@ enum KvKind : uint32_t { kF16 = 0, kBF16 = 1, kFP8 = 2, kFP4 = 3 };
 constexpr int kBlockSize = 16;          // tokens per page (engine/engine.bm:102)
 constexpr int kMaxBatchPerLaunch = 1024; // sequences per decode launch (prefix tables in smem)
 constexpr int kMinPagesPerCta = 8;      // work quantum when the batch is tiny
+constexpr int kPrefillTileRows = 128;   // query rows of a grouped prefill's tile
 constexpr int kMaxSegmentCost = 64;     // bound of DecodeParams::seg_cost
 constexpr uint32_t kMaxWindow = 1u << 30;   // windows and sinks are clamped to it (positions stay below)
 
@@ -98,9 +99,8 @@ struct PrefillParams {
     // are ones that nothing completes and run out
     uint64_t wait_cycles;
     uint32_t window, sinks;     // window > 0: the mask of PageSpan (both at most kMaxWindow)
-    float* part_o;              // [part_tiles][128][D] split-K partial outputs (grouped kernel)
-    float* part_ml;             // [part_tiles][128][2] (running max, sum)
-    uint32_t part_tiles;
+    float* part_o;              // [sms][kPrefillTileRows][D] split-K partial outputs (grouped kernel)
+    float* part_ml;             // [sms][kPrefillTileRows][2] (running max, sum)
 };
 
 struct PrefillLaunch {

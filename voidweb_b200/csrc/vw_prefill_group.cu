@@ -44,7 +44,7 @@ namespace vw {
 
 namespace {
 
-constexpr int kGRows = 128;                       // query rows per CTA
+constexpr int kGRows = kPrefillTileRows;          // query rows per CTA
 constexpr int kGKeys = 64;                        // keys per round
 constexpr int kGPages = kGKeys / kBlockSize;
 constexpr int kMaxSplit = 8;
@@ -785,13 +785,13 @@ cudaError_t launch_grp(const PrefillLaunch& L) {
     const PrefillParams& p = L.p;
     // an upper bound on the CTAs: sum over b of ceil(n_b * group / 128) <= T * group / 128 + B
     const uint64_t ctas = ((uint64_t)p.T * p.group + kGRows - 1) / kGRows + p.B;
-    // Parts of a tile: while there is an SM for each, the scratch holds them, and a block-table
+    // Parts of a tile: while there is an SM (and a tile of scratch) for each, and a block-table
     // row holds kMinRounds rounds for each.  (Llama-3-8B heads, 32 tokens behind 8192:
     // 130.6 us whole, 32.7 in eight parts.  Two CTAs on an SM slow one another, so
     // with two parts of 112 tiles, 40 tokens behind 1500 of 7 sequences, 40.2 us against
     // 33.8 whole.)
     const uint64_t tiles = ctas * p.Hkv, row_rounds = (p.bt_stride + kGPages - 1) / kGPages;
-    uint64_t splits = std::min<uint64_t>(L.sms, p.part_tiles) / tiles;
+    uint64_t splits = (uint64_t)L.sms / tiles;
     splits = std::min<uint64_t>({splits, kMaxSplit, row_rounds / kMinRounds});
     if (splits < 1) splits = 1;
     cudaLaunchConfig_t cfg = {};
