@@ -73,3 +73,49 @@ def test_reads_what_an_unsplit_decode_appended(kv, io, D, Hq, Hkv, window):
             ref = attend(q2[s:s + 1].cpu(), held(bt.k[s], kv), held(bt.v[s], kv), torch.tensor([totals[s] - 1]), window, 1 if window else 0)
             check(got["prefill"][1][s:s + 1], *ref, io, kv, f"prefill {s}")
             check(got["decode"][2][s:s + 1], *ref, io, kv, f"decode {s}")
+
+
+@pytest.mark.parametrize("n", [9, 700], ids=["split", "whole"])
+@pytest.mark.parametrize("kv,io,D,Hq,Hkv,window", KINDS)
+def test_decodes_and_prefills_in_turn(kv, io, D, Hq, Hkv, window, n):
+    """Layers of a mixed step: a decode with fused append, the prefill of another sequence's chunk (over cached rows, then over
+    rows that the call appends), all dependent launches, each prefill's queries the outputs of the launch before it; the bits
+    of the same calls made one after the other."""
+    from voidweb_b200 import _lib as C
+    L, totals = 3, [3000, 40, 7, 900]
+    win = dict(window=window * 30, sinks=1) if window else {}
+    a, b = (Batch(32, kv, io, D, Hq, Hkv, totals, layers=L).fill([totals[0] - n, 39, 6, 899]) for _ in range(2))
+    q = a.rows(3, Hq).to(a.dev)
+    kn, vn = (torch.stack([x[-1] for x in y[1:]]).to(a.dev) for y in (a.k, a.v))
+    kc, vc = (y[0][-n:].to(a.dev) for y in (a.k, a.v))
+    cu, start = torch.tensor([0, n], dtype=torch.int32, device=a.dev), a.lens()[:1] - n
+    before = torch.tensor([0, 3], dtype=torch.int32, device=a.dev), a.lens()[:1] - n - 3     # the three tokens before the chunk
+    q0, results = a.rows(n, Hq).to(a.dev), []
+    for bt, chained in ((a, False), (b, True)):
+        t, lens = bt.device_table(), bt.lens()
+        t0, t1, l1 = t[:1].contiguous(), t[1:].contiguous(), lens[1:].contiguous()
+        outs = [[torch.full_like(x, 7.0) for x in (q, q, q0, q0)] for _ in range(L)]
+        pdl = C.VW_PREFILL_PDL if chained else 0
+        qc = q0
+        torch.cuda.synchronize()
+
+        def done():
+            if not chained:
+                torch.cuda.synchronize()
+
+        for l, (dec, mid, pre, again) in enumerate(outs):
+            flags = (C.VW_DECODE_PDL | C.VW_DECODE_EARLY_PAGES) if chained and l else C.VW_DECODE_PDL if chained else 0
+            bt.pool.paged_decode(l, q, t1, l1, dec, k_new=kn, v_new=vn, flags=flags, **win)
+            done()
+            bt.pool.paged_prefill(l, dec, *before, t0, mid, flags=pdl, **win)
+            done()
+            bt.pool.paged_prefill(l, qc, cu, start, t0, pre, k_new=kc, v_new=vc, flags=pdl, **win)
+            done()
+            bt.pool.paged_prefill(l, pre, cu, start, t0, again, flags=pdl, **win)
+            done()
+            qc = again
+        assert bt.pool.check() == 0
+        results.append([x for o in outs for x in o])
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+    assert torch.equal(a.pool.pages_u8(), b.pool.pages_u8())
+    assert all(x.isfinite().all() for x in results[0])
