@@ -472,9 +472,10 @@ uint32_t env_decode_flags() {
 // pages 18 (the Qwen2.5-7B batch-16 step 4658 GB/s against 4531 at 12, 4665
 // at 21, 4609 at 24, 4032 at 6; the Llama-3-70B one-KV-head batch 6265
 // against 6290 at 12 and 6244 at 24), FP8 pages 12 (the Llama-3-8B batch 4062
-// against 3995 at 0, 4081 at 6, 3996 at 18), 4-bit pages 24 (a Llama-3-8B
-// batch of 64 with 1k to 16k tokens 110.5 us a layer against 126.1 at 0, 112.4 at
-// 18, 112.1 at 32, 116.3 at 48).
+// against 3995 at 0, 4081 at 6, 3996 at 18), 4-bit pages 32 (a Llama-3-8B
+// batch of 64 with 1k to 16k tokens 96.1 us a layer against 110.0 at 0, 102.7 at 12,
+// 98.1 at 24, 96.4 at 48; Qwen2.5-7B heads, 16 sequences of 512 to 4096, 14.1
+// against 16.9 at 0, 15.8 at 12, 14.8 at 24, 14.5 at 48).
 // VOIDWEB_KV_SEGMENT_COST=n overrides it (at most kMaxSegmentCost).
 uint32_t segment_cost(const PoolGeom& g) {
     static const long env = [] {
@@ -482,7 +483,7 @@ uint32_t segment_cost(const PoolGeom& g) {
         return e ? std::strtol(e, nullptr, 10) : -1L;
     }();
     if (env >= 0) return (uint32_t)std::min<long>(env, kMaxSegmentCost);
-    return g.kv_kind == kFP4 ? 24u : g.kv_kind == kFP8 ? 12u : 18u;
+    return g.kv_kind == kFP4 ? 32u : g.kv_kind == kFP8 ? 12u : 18u;
 }
 
 static int32_t decode_launch(vw_pool* pool, const vw_decode_args* a, cudaStream_t s,
