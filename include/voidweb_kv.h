@@ -34,6 +34,16 @@
  *         row share the scale s = E4M3(amax / 6); each is the E2M1 code of x / s
  *         (both to nearest even, saturating; a group whose s rounds to 0 holds
  *         zeros) and stands for code * s, which f16 and bf16 hold exactly.
+ *         There is no factor above a group's scale, so a group's largest magnitude
+ *         wants to lie between 0.094 and 2688: larger elements saturate, below
+ *         0.094 the scale is subnormal and keeps three bits or fewer, and at
+ *         6 * 2^-10 (0.0059) or less the group is held as zeros.  Rows of other
+ *         magnitudes can be multiplied by a power of two before they are
+ *         appended, and the softmax scale (K) and the outputs (V) divided by it.
+ * Queries: over FP8 pages they enter the products as f16, so a bf16 element of
+ * 65,536 or more becomes infinite and those below 2^-14 lose bits; over the other
+ * pages every row of the io type's range holds (4-bit pages: to 2^-24 of the row's
+ * largest element).
  */
 #ifndef VOIDWEB_KV_H
 #define VOIDWEB_KV_H
@@ -159,7 +169,8 @@ typedef struct {
  * also the append of the step's token (one launch per layer).  Device pointers;
  * all of them 16-byte aligned.  Calls on one stream are ordered; calls of one
  * pool on different streams must not run at the same time (they share the
- * pool's split-K scratch). */
+ * pool's split-K scratch).  A batch of no sequences returns VW_OK, its pointers
+ * NULL or not. */
 VW_API int32_t vw_paged_decode(vw_pool* pool, const vw_decode_args* args, void* stream);
 
 /* Sliding-window attention with sinks (no reference kernel).  A query at
@@ -169,7 +180,8 @@ VW_API int32_t vw_paged_decode(vw_pool* pool, const vw_decode_args* args, void* 
  * Pages without a visible key are neither resolved nor read, so their
  * block-table entries may hold anything (e.g. ids of blocks given back).
  * Every row sees its own token, so no row is empty.  Under a window, and over
- * 4-bit pools, block_table_stride is at most 2^26 (2^30 tokens). */
+ * 4-bit pools, block_table_stride is at most 2^26 (2^30 tokens).  A call without a
+ * window is the plain entry point; voidweb_forward_pass and vw_sched have none. */
 typedef struct {
     uint32_t window;
     uint32_t sinks;
@@ -256,7 +268,7 @@ typedef struct {
     float rope_theta;              /* > 0: fused RoPE on q and the new K rows (VW_DECODE_ROPE) */
 } vw_step_host_args;
 VW_API int32_t vw_decode_step_host(vw_pool* pool, const vw_step_host_args* args, void* stream);
-/* The same step with every layer's decode under one window. */
+/* The same step with every layer's decode under one window (the same for all). */
 VW_API int32_t vw_decode_step_host_window(vw_pool* pool, const vw_step_host_args* args,
                                           const vw_window* window, void* stream);
 
@@ -272,8 +284,9 @@ VW_API int32_t vw_decode_step_host_window(vw_pool* pool, const vw_step_host_args
  * then token i attends to keys 0 .. ctx_start[b]+i with VW_PREFILL_CAUSAL, or
  * to all ctx_start[b] + n_b keys without it (the reference kernel has no mask).
  * Every pool kind: f16 / bf16 pages (head_dim 64 or 128) and FP8 E4M3 pages
- * (head_dim 128; attention over the dequantised codes).  Device pointers,
- * 16-byte aligned (the int arrays 4-byte). */
+ * (head_dim 128; attention over the dequantised codes), and 4-bit pages.  Device
+ * pointers, 16-byte aligned (the int arrays 4-byte).  No sequences or no tokens:
+ * VW_OK, the pointers NULL or not. */
 typedef struct {
     uint32_t layer;
     uint32_t num_seqs;             /* B, at most the pool's max_batch */

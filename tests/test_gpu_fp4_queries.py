@@ -119,3 +119,23 @@ def test_rotated_rows(D, Hq, Hkv):
         x, y = got[0][i].double(), got[20][i].double()
         tol = 2 * (2.0 ** -8 * 1.01 * (x.abs() + 2.0 ** -8 * most) + (2.0 ** -11 + 2.0 ** -13) * most + 2.0 ** -25 * max(LENS) * most)
         assert ((x - y).abs() <= tol).all()
+
+
+def test_small_rows_by_powers_of_two():
+    """Rows below the format's scales, held as a user can: multiplied by a power of two on the way in, the softmax scale and the
+    outputs divided by it.  The same bits as the rows at their ordinary size give."""
+    ordinary = Batch(5, "fp4", "bf16", 128, 8, 2, LENS).fill()
+    small = Batch(5, "fp4", "bf16", 128, 8, 2, LENS)
+    k, v = [times(x, -9) for x in small.k], [times(x, -12) for x in small.v]           # the model's rows
+    assert (held(v[3], "fp4") == 0).all() and (held(k[3], "fp4") == 0).float().mean() > 0.5
+    small.k, small.v = [times(x, 9) for x in k], [times(x, 12) for x in v]             # what is appended
+    small.fill()
+    q = ordinary.rows(4, 8).to(ordinary.dev)
+    a, b = torch.zeros_like(q), torch.zeros_like(q)
+    ordinary.pool.paged_decode(0, q, ordinary.device_table(), ordinary.lens(), a)
+    small.pool.paged_decode(0, q, small.device_table(), small.lens(), b, scale=1 / math.sqrt(128))
+    assert ordinary.pool.check() == small.pool.check() == 0
+    assert torch.equal(times(a, -12), times(b, -12))
+    r = refs(small, q.cpu()[:, None], [torch.tensor([n - 1]) for n in LENS], 0, 1 / math.sqrt(128))
+    for i in range(4):
+        check(b[i:i + 1], *r[i], "bf16", "fp4", f"sequence {i}")

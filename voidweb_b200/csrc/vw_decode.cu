@@ -47,8 +47,8 @@
 //    and the probabilities.
 //  * Windows (vw_window.cuh).  The pages without a visible key are left out of the
 //    split and never resolved; a page that a window or the sinks cut is masked.  16
-//    sequences of Qwen2.5-7B under a window of 4096 tokens: 26.4 us a layer
-//    (119 MB, 4.5 TB/s); 64 of Llama-3-8B over FP8 pages: 121 us (443 MB, 3.7 TB/s,
+//    sequences of Qwen2.5-7B under a window of 4096 tokens: 26.2 us a layer
+//    (119 MB, 4.5 TB/s); 64 of Llama-3-8B over FP8 pages: 119 us (443 MB, 3.7 TB/s,
 //    bound by the expansion of the codes as without a window).
 //
 // Every wait is bounded (vw_ptx.cuh); on timeout the kernel records

@@ -21,13 +21,17 @@
 //    page and those a window cuts go one at a time.
 //  * Online softmax in the log2 domain with a lazily raised maximum (a score must
 //    exceed it by 8 before it is raised); sums and outputs in f32.
-//    Probabilities enter P V as one f16, relative error 2^-12 at most, 2^-25 below
-//    2^-14: it adds some 1e-4 to the result's relative error, whose rounding to the
-//    io type is 2e-4 (f16) or 1.7e-3 (bf16) in the root mean square, and saves a
-//    quarter of the matrix instructions.
-//  * Measured: Llama-3-8B heads, 64 sequences of 1024 to 16,384 tokens, 96.5 us a layer (4.1
+//    Probabilities enter P V as one f16, off by at most 2^-11 of themselves, 2^-25 below
+//    2^-14: the results' relative error, in the root mean square, becomes 2.4e-4 to
+//    2.8e-4 in f16, whose own rounding is 2.1e-4, and stays at 1.7e-3 in bf16; it saves
+//    a quarter of the matrix instructions.
+//  * bf16 queries go into f16 by rows (fp4_query_factor), so that no value of theirs is lost.
+//  * Two CTAs of eight warps and 128 registers fill the register file (with two query-head
+//    tiles, 64,512 of it), so the combine's CTAs come up as decode CTAs leave, not beside
+//    them; the D 128 instances spill 32 to 44 B besides.
+//  * Measured: Llama-3-8B heads, 64 sequences of 1024 to 16,384 tokens, 96.1 us a layer (4.2
 //    TB/s; 325 instructions per page-head, ALU 51 %, and some 17 us of 512 segments'
-//    starts and merges); Qwen2.5-7B heads, 16 sequences of 512 to 4096, 14.4 us.
+//    starts and merges); Qwen2.5-7B heads, 16 sequences of 512 to 4096, 14.1 us.
 #include <cuda_runtime.h>
 #include <atomic>
 #include <cstdint>
@@ -498,7 +502,7 @@ __global__ void __launch_bounds__(T::THREADS, 2) fp4_decode_kernel(const DecodeP
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
     constexpr int W = T::W, NTH = T::THREADS;
     // Programmatic dependent launch, as in vw_decode.cu: without early pages
-    // everything waits for the predecessor; the combine may launch at once.
+    // everything waits for the predecessor; the combine may launch as soon as it finds room.
     const bool pdl = (p.flags & kDecodePdl) != 0, early = pdl && (p.flags & kDecodeEarlyPages) != 0;
     if (pdl && !early) griddep_wait();
     griddep_launch_dependents();

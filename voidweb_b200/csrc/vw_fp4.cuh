@@ -97,9 +97,10 @@ __device__ __forceinline__ uint32_t fp4_encode4(const float* v, float inverse) {
 }
 
 // Eight codes of a word -> four f16 pairs (exact).  The word is one that its lane
-// loaded whole, or a bitwise mix of such words: ptxas 12.9 turned the byte
-// conversions of a kernel parameter (a uniform register) into an instruction that
-// raised "misaligned address", and those of a zero-extended 16-bit value into zeros.
+// loaded whole, or a bitwise mix of such words.  Under ptxas 12.9 a kernel that
+// converted the bytes of its own parameter (perhaps from a uniform register) raised
+// "misaligned address", and the bytes of a zero-extended 16-bit value became zeros;
+// why is not known.
 __device__ __forceinline__ void fp4x8_to_f16(uint32_t w, uint32_t (&r)[4]) {
     asm("{\n\t.reg .b8 a, b, c, d;\n\t"
         "mov.b32 {a, b, c, d}, %4;\n\t"

@@ -867,7 +867,10 @@ cudaError_t launch_w(const PrefillLaunch& L) {
 }
 
 // Windows: FP8 pools have an instance of their own here, the others the grouped kernel
-// (vw_prefill_group.cu).
+// (vw_prefill_group.cu), which has no warps that expand FP8 codes.  Here every query head
+// of a group expands its KV head's codes for itself and masks most of 128 + window
+// keys: Llama-3-8B heads, 4 chunks of 2048 tokens behind 0 to 8192, window 1024 624 us
+// (bf16 pages, grouped: 182), window 4096 1480 us (379).
 template <class T>
 cudaError_t launch_t(const PrefillLaunch& L) {
     if constexpr (T::FP8) {

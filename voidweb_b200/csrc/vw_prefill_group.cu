@@ -21,8 +21,8 @@
 //    walks all its keys, some 1.1 us per round: the rounds of a tile are then split over
 //    up to kMaxSplit CTAs, which leave unnormalised outputs with their maxima and sums
 //    in f32, and a small grid merges them.
-//  * Measured, Qwen2.5-7B heads, 4 chunks of 2048 tokens: under a window of 1024 tokens 187 us
-//    (570 TFLOP/s of visible work; of some 2300 cycles of a pair of rounds the matrix
+//  * Measured, Qwen2.5-7B heads, 4 chunks of 2048 tokens: under a window of 1024 tokens 176 to
+//    187 us (570 to 606 TFLOP/s of visible work; of some 2300 cycles of a pair of rounds the matrix
 //    instructions take 2032), over 4-bit pages 227 us (581 TFLOP/s; the softmax and the
 //    decoders set the pace).
 //  * Every wait is bounded; on timeout the kernel records kDevErrTimeout, waits
@@ -787,7 +787,7 @@ cudaError_t launch_grp(const PrefillLaunch& L) {
     const uint64_t ctas = ((uint64_t)p.T * p.group + kGRows - 1) / kGRows + p.B;
     // Parts of a tile: while there is an SM (and a tile of scratch) for each, and a block-table
     // row holds kMinRounds rounds for each.  (Llama-3-8B heads, 32 tokens behind 8192:
-    // 130.6 us whole, 32.7 in eight parts.  Two CTAs on an SM slow one another, so
+    // 130.6 us whole, 32.8 in eight parts.  Two CTAs on an SM slow one another, so
     // with two parts of 112 tiles, 40 tokens behind 1500 of 7 sequences, 40.2 us against
     // 33.8 whole.)
     const uint64_t tiles = ctas * p.Hkv, row_rounds = (p.bt_stride + kGPages - 1) / kGPages;

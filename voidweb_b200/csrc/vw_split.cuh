@@ -176,8 +176,10 @@ __device__ __forceinline__ void merge_unit(const DecodeParams& p, int b, int h, 
 // register file is split over the SM's four sub-partitions (16,384 each); ten
 // 128-register decode warps leave 4,096 in a sub-partition holding three of
 // them, so a combine CTA is a single warp of at most 80 registers (2,560),
-// and it runs with the decode's shared-memory carveout.  CTA (segment, j) merges query head j of the
-// segment, four output elements per lane.
+// and it runs with the decode's shared-memory carveout.  (The decode of 4-bit pools leaves no
+// such room: its two CTAs take the whole register file, and its combine starts as
+// they leave.)  CTA (segment, j) merges query head j of the segment, four output
+// elements per lane.
 constexpr int kCombineWarps = 1;
 constexpr int kCombineThreads = kCombineWarps * 32;
 constexpr int kCombineMinBlocks = 25;  // 65,536 / (32 x 25) -> a cap of 80 registers
@@ -185,7 +187,7 @@ constexpr int kCombineMinBlocks = 25;  // 65,536 / (32 x 25) -> a cap of 80 regi
 // Merge of the split-K partials, one CTA per (sequence, KV head) segment.  The
 // CTA recomputes the decode grid's page ranges from seq_lens (same clamping,
 // same per-CTA quantum), returns at once for a segment that one decode CTA
-// finished, and otherwise merges the pieces (o, max, sum) left by decode CTAs
+// finished (CTA 0 waits all the same), and otherwise merges the pieces (o, max, sum) left by decode CTAs
 // c0..c1 with weights 2^(max_c - max) -- the merge rule of the online softmax
 // in flash_attention.bm:149-157, applied across pieces instead of tokens.
 // Launched as a programmatic dependent of its decode grid: the geometry is
