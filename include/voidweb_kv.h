@@ -34,6 +34,7 @@
  *         row share the scale s = E4M3(amax / 6); each is the E2M1 code of x / s
  *         (both to nearest even, saturating; a group whose s rounds to 0 holds
  *         zeros) and stands for code * s, which f16 and bf16 hold exactly.
+ *         A NaN element is held as 6 * s and does not count in amax.
  *         There is no factor above a group's scale, so a group's largest magnitude
  *         wants to lie between 0.094 and 2688: larger elements saturate, below
  *         0.094 the scale is subnormal and keeps three bits or fewer, and at
