@@ -119,3 +119,27 @@ def test_decodes_and_prefills_in_turn(kv, io, D, Hq, Hkv, window, n):
     assert all(torch.equal(x, y) for x, y in zip(*results))
     assert torch.equal(a.pool.pages_u8(), b.pool.pages_u8())
     assert all(x.isfinite().all() for x in results[0])
+
+
+@pytest.mark.parametrize("kv,io,D,Hq,Hkv,window", KINDS)
+def test_host_step_of_an_unsplit_batch(kv, io, D, Hq, Hkv, window):
+    """The read-back of a layer's outputs follows its combine: direct, recorded and replayed steps read finished outputs."""
+    L, totals = 4, [1 + i % 16 for i in range(300)]
+    a, b = (Batch(33, kv, io, D, Hq, Hkv, totals, layers=L, max_batch=300).fill([n - 1 for n in totals]) for _ in range(2))
+    q = torch.stack([a.rows(a.B, Hq) for _ in range(L)]).pin_memory()
+    kn, vn = (torch.stack([torch.stack([x[-1] for x in y])] * L).pin_memory() for y in (a.k, a.v))
+    table, lens = a.device_table().cpu().pin_memory(), a.lens().cpu().pin_memory()
+    win = dict(window=window, sinks=1) if window else {}
+    want = torch.zeros_like(q)
+    for l in range(L):
+        o = torch.zeros_like(q[l]).to(b.dev)
+        b.pool.paged_decode(l, q[l].to(b.dev), b.device_table(), b.lens(), o, k_new=kn[l].to(b.dev), v_new=vn[l].to(b.dev), **win)
+        torch.cuda.synchronize()
+        want[l] = o.cpu()
+    out = torch.zeros_like(q).pin_memory()
+    for _ in range(6):
+        out.fill_(7.0)
+        a.pool.decode_step_host(q, kn, vn, table, lens, out, **win)
+        assert torch.equal(out, want)
+    assert a.pool.check() == b.pool.check() == 0
+    assert torch.equal(a.pool.pages_u8(), b.pool.pages_u8())
